@@ -26,6 +26,9 @@ NVCC_FLAGS = [
     "--use_fast_math", "-Xcompiler", "-fPIC", "-Xptxas", "-v",
 ]
 
+# Compiled without --use_fast_math: a table's or a gradient's subnormal values are kept, divisions and square roots are rounded.
+PRECISE = {"token_table", "orthogonalize"}
+
 
 def _nvcc() -> str:
     cand = shutil.which("nvcc") or "/usr/local/cuda/bin/nvcc"
@@ -70,7 +73,7 @@ def build(force: bool = False, verbose: bool = False) -> Path:
         obj = BUILD / (src.stem + ".o")
         objs.append(obj)
         if force or _stale(obj, [src] + headers):
-            jobs.append(([_nvcc(), *NVCC_FLAGS, "-I", str(CSRC), "-c", str(src), "-o", str(obj)],
+            jobs.append(([_nvcc(), *(f for f in NVCC_FLAGS if f != "--use_fast_math" or src.stem not in PRECISE), "-I", str(CSRC), "-c", str(src), "-o", str(obj)],
                          BUILD / (src.stem + ".log")))
     for src in cpp_files:
         obj = BUILD / (src.stem + ".o")

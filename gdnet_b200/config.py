@@ -1,7 +1,7 @@
 """Training configuration: a dataclass loaded from YAML with unknown keys rejected.
 
 Keys and defaults follow the reference's ``Config`` (scripts/training.py:52-106) so its YAML
-files load unchanged; the extra keys (``fp8_recipe``, ``comm``, ``engine``, ``wait_budget_s``,
+files load unchanged; the extra keys (``fp8_recipe``, ``comm``, ``matrix_optimizer``, ``engine``, ``wait_budget_s``,
 ``heartbeat_dir``) select B200-specific behaviour and all have defaults.
 """
 
@@ -59,6 +59,7 @@ class Config:
     fp8_recipe: str = "block"          # block | tensor
     comm: str = "fused"                # fused (peer-memory kernels) | scatter (reduce-scatter in the GEMM epilogues) | nccl
     shard: str = "none"                # none | full (layer matrices, gradients and AdamW moments spread over the ranks)
+    matrix_optimizer: str = "adamw"    # adamw | muon (layer matrices along their orthogonalised momentum; one GPU or comm nccl)
     engine: bool = True                # flat-buffer engine on CUDA; False = generic optimizer path
     wait_budget_s: float = 2.0         # documented bound of every in-kernel wait
     heartbeat_dir: str = ""            # per-rank heartbeat files for the watchdog ("" = off)

@@ -8,11 +8,13 @@
 
 #include <nvtx3/nvToolsExt.h>
 
+#include <algorithm>
 #include <cstdlib>
 
 #include "comm.h"
 #include "gemm_sm100.h"
 #include "kernels.h"
+#include "orthogonalize.h"
 
 namespace {
 
@@ -1067,6 +1069,172 @@ void halo_push_wait(const Tensor& tail, Tensor halo_out, const Tensor& slot_ptrs
   GD_LAUNCH(gd::launch_halo_push_wait(a, stream_of(tail)));
 }
 
+// ---- token table ------------------------------------------------------------------------------
+int elem_type(const Tensor& t, const char* name) {
+  switch (t.scalar_type()) {
+    case at::kBFloat16: return gd::ELEM_BF16;
+    case at::kHalf: return gd::ELEM_F16;
+    case at::kFloat: return gd::ELEM_F32;
+    default: TORCH_CHECK(false, name, " must be bfloat16, float16 or float32");
+  }
+}
+
+void check_tokens(const Tensor& tokens, const Tensor& like) {
+  TORCH_CHECK(tokens.is_cuda() && tokens.device() == like.device(), "tokens must be on the same CUDA device");
+  TORCH_CHECK(tokens.scalar_type() == at::kLong || tokens.scalar_type() == at::kInt, "tokens must be int64 or int32");
+  TORCH_CHECK(tokens.is_contiguous(), "tokens must be contiguous");
+}
+
+void token_lookup(const Tensor& tokens, const Tensor& table, double scale, Tensor out) {
+  c10::cuda::CUDAGuard guard(table.device());
+  OpRange gd_range_(__func__);
+  check_cuda(table, "table");
+  check_cuda(out, "out");
+  check_tokens(tokens, table);
+  TORCH_CHECK(table.dim() == 2 && out.is_contiguous() && out.scalar_type() == table.scalar_type() &&
+              out.device() == table.device() && out.numel() == tokens.numel() * table.size(1), "token_lookup: out must be (tokens, width) of the table's type");
+  gd::TokenLookupArgs a{};
+  a.tokens = tokens.data_ptr();
+  a.wide = tokens.scalar_type() == at::kLong;
+  a.n = tokens.numel();
+  a.table = table.data_ptr();
+  a.vocab = table.size(0);
+  a.width = table.size(1);
+  a.ld = table.stride(0);
+  a.dtype = elem_type(table, "table");
+  a.scale = (float)scale;
+  a.out = out.data_ptr();
+  GD_LAUNCH(gd::launch_token_lookup(a, status_ptr(table), stream_of(table)));
+}
+
+void token_grad(const Tensor& tokens, const Tensor& grad, double scale, bool add, Tensor out) {
+  c10::cuda::CUDAGuard guard(grad.device());
+  OpRange gd_range_(__func__);
+  check_cuda(grad, "grad");
+  check_cuda(out, "out");
+  check_tokens(tokens, grad);
+  TORCH_CHECK(grad.dim() == 2 && out.dim() == 2 && out.is_contiguous() && out.device() == grad.device() &&
+              grad.size(0) == tokens.numel() && out.size(1) == grad.size(1), "token_grad: grad is (tokens, width), out (vocab, width)");
+  TORCH_CHECK(out.scalar_type() == (add ? at::kFloat : grad.scalar_type()), "token_grad: out has the wrong type");
+  if (!add) out.zero_();
+  const auto words = at::TensorOptions().device(grad.device());
+  const int64_t n = tokens.numel();
+  Tensor sort = at::empty({4 * n}, words.dtype(at::kInt));
+  Tensor partial = at::empty({gd::token_grad_partial_floats(n, grad.size(1))}, words.dtype(at::kFloat));
+  gd::TokenGradArgs a{};
+  a.tokens = tokens.data_ptr();
+  a.wide = tokens.scalar_type() == at::kLong;
+  a.n = n;
+  a.grad = grad.data_ptr();
+  a.vocab = out.size(0);
+  a.width = grad.size(1);
+  a.grad_ld = grad.stride(0);
+  a.dtype = elem_type(grad, "grad");
+  a.scale = (float)scale;
+  a.add = add;
+  a.out = out.data_ptr();
+  a.sort = reinterpret_cast<uint32_t*>(sort.data_ptr());
+  a.partial = partial.data_ptr<float>();
+  GD_LAUNCH(gd::launch_token_grad(a, status_ptr(grad), stream_of(grad)));
+}
+
+// ---- Newton-Schulz ------------------------------------------------------------------------------
+// Matrices per launch group: at most NS_MAX_BATCH, and at most 2^26 elements (about 0.6 GB of workspace), in groups of equal size.
+int64_t ns_group(int64_t n, int64_t rows, int64_t cols) {
+  const int64_t most = std::max<int64_t>(1, std::min<int64_t>(gd::NS_MAX_BATCH, (int64_t(1) << 26) / (rows * cols)));
+  const int64_t groups = (n + most - 1) / most;
+  return (n + groups - 1) / groups;
+}
+
+void ns_setup(gd::NsCall& call, int64_t rows, int64_t cols, int64_t steps, at::ArrayRef<double> c, double eps, bool pairs) {
+  TORCH_CHECK(c.size() == 3 && steps >= 0 && steps <= 1000, "orthogonalize: steps and coefficients");
+  TORCH_CHECK(rows <= (1 << 20) && cols <= (1 << 20), "orthogonalize: matrix too large");
+  call.ends.rows = (int)rows;
+  call.ends.cols = (int)cols;
+  call.ends.eps = (float)eps;
+  call.steps = (int)steps;
+  call.pairs = pairs;
+  for (int i = 0; i < 3; ++i) call.c[i] = (float)c[i];
+}
+
+void orthogonalize(const Tensor& x, Tensor out, int64_t steps, at::ArrayRef<double> c, double eps, bool pairs) {
+  c10::cuda::CUDAGuard guard(x.device());
+  OpRange gd_range_(__func__);
+  check_cuda(x, "x");
+  check_cuda(out, "out");
+  TORCH_CHECK(x.dim() == 3 && out.sizes() == x.sizes() && out.is_contiguous() && out.device() == x.device(), "orthogonalize: (n, rows, cols) tensors");
+  const int64_t n = x.size(0), rows = x.size(1), cols = x.size(2);
+  if (x.numel() == 0) return;
+  gd::NsCall call{};
+  ns_setup(call, rows, cols, steps, c, eps, pairs);
+  call.ends.grad_dtype = elem_type(x, "x");
+  call.ends.out_dtype = elem_type(out, "out");
+  call.ends.grad_ld = x.stride(1);
+  const int64_t group = ns_group(n, rows, cols);
+  Tensor space = at::empty({gd::ns_workspace_bytes(group, rows, cols)}, x.options().dtype(at::kByte));
+  call.workspace = space.data_ptr();
+  for (int64_t i0 = 0; i0 < n; i0 += group) {
+    const int64_t count = std::min(group, n - i0);
+    call.ends.batch = (int)count;
+    for (int64_t i = 0; i < count; ++i) {
+      call.ends.grad[i] = reinterpret_cast<const char*>(x.data_ptr()) + (i0 + i) * x.stride(0) * x.element_size();
+      call.ends.out[i] = reinterpret_cast<char*>(out.data_ptr()) + (i0 + i) * rows * cols * out.element_size();
+    }
+    GD_LAUNCH(gd::launch_orthogonalize(call, status_ptr(x), stream_of(x)));
+  }
+}
+
+void muon_update(at::TensorList params, at::TensorList grads, at::TensorList infos, at::TensorList moments, OptT scalars,
+                 double beta, double mu, bool nesterov, double decay, double step, int64_t steps, at::ArrayRef<double> c, double eps,
+                 bool pairs) {
+  const int64_t n = (int64_t)params.size();
+  if (n == 0) return;
+  const Tensor& first = params[0];
+  c10::cuda::CUDAGuard guard(first.device());
+  OpRange gd_range_(__func__);
+  TORCH_CHECK((int64_t)grads.size() == n && (int64_t)moments.size() == n && (infos.empty() || (int64_t)infos.size() == n), "muon_update: one entry per matrix");
+  TORCH_CHECK(first.dim() == 2, "muon_update: matrices");
+  for (int64_t i = 0; i < n; ++i) {
+    const Tensor* ts[4] = {&params[i], &grads[i], &moments[i], infos.empty() ? &grads[i] : &infos[i]};
+    for (const Tensor* t : ts)
+      TORCH_CHECK(t->is_cuda() && t->device() == first.device() && t->is_contiguous() && t->sizes() == first.sizes(),
+                  "muon_update: contiguous matrices of one shape on one device");
+    TORCH_CHECK(params[i].scalar_type() == first.scalar_type() && grads[i].scalar_type() == grads[0].scalar_type() &&
+                (infos.empty() || infos[i].scalar_type() == grads[0].scalar_type()) && moments[i].scalar_type() == at::kFloat,
+                "muon_update: params and gradients of one type each, momentum in float32");
+  }
+  const int64_t rows = first.size(0), cols = first.size(1);
+  if (rows == 0 || cols == 0) return;
+  gd::NsCall call{};
+  ns_setup(call, rows, cols, steps, c, eps, pairs);
+  call.ends.momentum = 1;
+  call.ends.nesterov = nesterov;
+  call.ends.grad_dtype = elem_type(grads[0], "grads");
+  call.ends.out_dtype = elem_type(first, "params");
+  call.ends.grad_ld = cols;
+  if (scalars.has_value()) TORCH_CHECK(scalars->numel() >= 2 && scalars->device() == first.device(), "muon_update: scalars");
+  call.ends.scalars = opt_f32(scalars, "scalars");
+  TORCH_CHECK(infos.empty() || call.ends.scalars != nullptr, "muon_update: information gradients need the projection scalars");
+  call.ends.beta = (float)beta;
+  call.ends.mu = (float)mu;
+  call.ends.decay = (float)decay;
+  call.ends.step = (float)step;
+  const int64_t group = ns_group(n, rows, cols);
+  Tensor space = at::empty({gd::ns_workspace_bytes(group, rows, cols)}, first.options().dtype(at::kByte));
+  call.workspace = space.data_ptr();
+  for (int64_t i0 = 0; i0 < n; i0 += group) {
+    const int64_t count = std::min(group, n - i0);
+    call.ends.batch = (int)count;
+    for (int64_t i = 0; i < count; ++i) {
+      call.ends.grad[i] = grads[i0 + i].data_ptr();
+      call.ends.info[i] = infos.empty() ? nullptr : infos[i0 + i].data_ptr();
+      call.ends.moment[i] = moments[i0 + i].data_ptr();
+      call.ends.out[i] = params[i0 + i].data_ptr();
+    }
+    GD_LAUNCH(gd::launch_orthogonalize(call, status_ptr(first), stream_of(first)));
+  }
+}
+
 }  // namespace
 
 TORCH_LIBRARY(gdnet_b200, m) {
@@ -1097,6 +1265,10 @@ TORCH_LIBRARY(gdnet_b200, m) {
   m.def("cross_entropy(Tensor(a!) logits, Tensor targets, Tensor(b!) row_loss, Tensor inv_count, int vocab, int ignore_index, float grad_scale, bool write_grad) -> ()", &cross_entropy);
   m.def("mem_read_fwd(Tensor q, Tensor gamma, Tensor e, Tensor tags, Tensor vals, Tensor alpha, Tensor(a!) w, Tensor(b!) out) -> ()", &mem_read_fwd);
   m.def("mem_read_bwd(Tensor d_out, Tensor q, Tensor gamma, Tensor e, Tensor tags, Tensor vals, Tensor w, Tensor alpha, Tensor(a!) d_q, Tensor(b!) d_gamma, Tensor(c!) d_e, Tensor(d!) d_tags, Tensor(e!) d_vals, Tensor(f!) d_alpha) -> ()", &mem_read_bwd);
+  m.def("token_lookup(Tensor tokens, Tensor table, float scale, Tensor(a!) out) -> ()", &token_lookup);
+  m.def("token_grad(Tensor tokens, Tensor grad, float scale, bool add, Tensor(a!) out) -> ()", &token_grad);
+  m.def("orthogonalize(Tensor x, Tensor(a!) out, int steps, float[] c, float eps, bool pairs) -> ()", &orthogonalize);
+  m.def("muon_update(Tensor(a!)[] params, Tensor[] grads, Tensor[] infos, Tensor(b!)[] moments, Tensor? scalars, float beta, float mu, bool nesterov, float decay, float step, int steps, float[] c, float eps, bool pairs) -> ()", &muon_update);
   m.def("grad_dots(Tensor gt, Tensor? gi, Tensor(a!) sums) -> ()", &grad_dots);
   m.def("projected_adamw(Tensor(a!) p, Tensor gt, Tensor? gi, Tensor(b!) m, Tensor(c!) v, Tensor scalars, float beta_proj, float lr, float beta1, float beta2, float eps, float weight_decay, int step) -> ()", &projected_adamw);
   m.def("batched_outer_add(Tensor dsts, Tensor ys, Tensor vecs, Tensor coef, Tensor rows, Tensor cols, int max_rows) -> ()", &batched_outer_add);

@@ -281,7 +281,8 @@ __device__ __forceinline__ void tma_store_2d(const CUtensorMap* m, uint32_t src,
 __device__ __forceinline__ void bulk_commit_group() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
 // Every bulk store this thread has committed has finished READING its shared-memory source.
 __device__ __forceinline__ void bulk_wait_read_all() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
-// All but the most recently committed bulk store of this thread have finished reading their shared-memory source.
+// Every bulk store this thread has committed is complete (its bytes are written).
+__device__ __forceinline__ void bulk_wait_all() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
 
 // Per-thread asynchronous copy of 8 bytes from global to shared memory (zeros when !valid; src must still be a
 // mapped address). The data is visible to the issuing thread after cp_async_wait_but<N>().

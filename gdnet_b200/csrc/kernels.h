@@ -305,4 +305,36 @@ const char* launch_batched_outer_add(float* const* dsts, const float* const* ys,
                                      const float* coef, const int* rows, const int* cols, int n_mats, int max_rows,
                                      cudaStream_t st);
 
+// ---- token table (token_table.cu) -------------------------------------------------------------
+enum ElemType : int { ELEM_BF16 = 0, ELEM_F16 = 1, ELEM_F32 = 2 };
+
+struct TokenLookupArgs {
+  const void* tokens;   // [n] int64 (wide) or int32
+  int wide;
+  int64_t n;
+  const void* table;    // (vocab, width), row pitch ld
+  int64_t vocab, width, ld;
+  int dtype;            // ElemType of the table and of out
+  float scale;
+  void* out;            // (n, width) contiguous
+};
+
+struct TokenGradArgs {
+  const void* tokens;   // [n] int64 (wide) or int32
+  int wide;
+  int64_t n;
+  const void* grad;     // (n, width), row pitch grad_ld
+  int64_t vocab, width, grad_ld;
+  int dtype;            // ElemType of grad
+  float scale;
+  int add;              // 1: out is fp32 and is added to; 0: out has grad's type, rows of absent ids are left as they are
+  void* out;            // (vocab, width) contiguous
+  uint32_t* sort;       // 4 n words
+  float* partial;       // token_grad_partial_floats()
+};
+
+const char* launch_token_lookup(const TokenLookupArgs& a, Status* status, cudaStream_t st);
+int64_t token_grad_partial_floats(int64_t n, int64_t width);
+const char* launch_token_grad(const TokenGradArgs& a, Status* status, cudaStream_t st);
+
 }  // namespace gd

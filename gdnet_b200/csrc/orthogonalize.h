@@ -1,0 +1,61 @@
+// Host-visible interface of the Newton-Schulz products (orthogonalize.cu).
+#pragma once
+
+#include <cuda.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include "kernels.h"
+
+namespace gd {
+
+constexpr int NS_MAX_BATCH = 64;       // matrices of one shape per call: their addresses travel in the kernel arguments
+constexpr int NS_NORM_BLOCKS = 64;     // partial sums of a matrix's norm
+
+// Element-wise ends of a call: what the matrices are made from and where the result goes.
+struct NsEnds {
+  int batch, rows, cols;
+  int ld;                              // row pitch of the workspace planes (elements)
+  int64_t plane;                       // elements of one workspace plane
+  const void* grad[NS_MAX_BATCH];      // input, or the (task) gradient
+  const void* info[NS_MAX_BATCH];      // information gradient, may be null
+  void* moment[NS_MAX_BATCH];          // fp32 momentum, updated in place (momentum != 0)
+  void* out[NS_MAX_BATCH];             // result, or the parameter, updated in place
+  int grad_dtype, out_dtype;           // ElemType
+  int64_t grad_ld;                     // row pitch of the input without momentum
+  const float* scalars;                // {projection coefficient, gradient scale} on the device, may be null
+  float beta, mu, eps, decay, step;
+  int momentum, nesterov;
+  float* u;
+  double* partial;
+  __half* x_hi;
+  __half* x_lo;
+};
+
+struct NsMaps {
+  CUtensorMap p_hi, p_lo, q_hi, q_lo, out_hi, out_lo;
+};
+
+// One product over the batch (see ns_product_body)
+struct NsProduct {
+  int batch, M, N, K;
+  int symmetric, pairs, p_mn, q_mn, store_lo;
+  int tiles, tiles_m;                  // tiles of one matrix; row blocks
+  float acc_scale, aux_scale;
+  const __half* aux_hi;
+  const __half* aux_lo;
+  int64_t aux_ld, aux_stride;
+};
+
+struct NsCall {
+  NsEnds ends;
+  void* workspace;                     // ns_workspace_bytes(), 256-byte aligned
+  int steps, pairs;
+  float c[3];                          // coefficients a, b, c of the step
+};
+
+int64_t ns_workspace_bytes(int64_t batch, int64_t rows, int64_t cols);
+const char* launch_orthogonalize(const NsCall& call, Status* status, cudaStream_t st);
+
+}  // namespace gd

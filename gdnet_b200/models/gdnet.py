@@ -25,7 +25,8 @@ class GDNet(nn.Module):
     """Gated Dissipative Network.
 
     Args mirror the reference (gdnet/model.py:35-72). ``cam_enabled`` and
-    ``trans_enabled`` start True.
+    ``trans_enabled`` start True. ``embed_scale`` (not in the reference) multiplies the looked-up token rows; the
+    tied vocabulary projection is not scaled.
     """
 
     def __init__(
@@ -41,6 +42,7 @@ class GDNet(nn.Module):
         n_slots: int = 32,
         kernel_size: int = 7,
         n_ops: int = 8,
+        embed_scale: float = 1.0,
     ) -> None:
         super().__init__()
         d_c = d_c or d // 4
@@ -60,6 +62,7 @@ class GDNet(nn.Module):
 
         self.vocab_size, self.vocab_padded = vocab_size, vocab_padded
         self.d, self.d_embed = d, d_embed
+        self.embed_scale = float(embed_scale)
         self.n_layers, self.n_cycles = n_layers, n_cycles
         self.chunk_size, self.kernel_size = chunk_size, kernel_size
         self.cam_enabled = True
@@ -72,7 +75,9 @@ class GDNet(nn.Module):
     # -- trunk ------------------------------------------------------------------------
 
     def _embed(self, tokens: torch.Tensor) -> torch.Tensor:
-        return self.proj_in(self.embed(tokens))
+        if type(self.embed) is nn.Embedding:
+            return self.proj_in(ops.embedding(tokens, self.embed.weight, self.embed_scale))
+        return self.proj_in(self.embed(tokens) * self.embed_scale)      # a wrapped or replaced table
 
     def one_cycle(self, fwd, side, sp_group=None, gate_sink=None, gate_mode=True, cycle=0):
         """All layers forward-step in order, then backward-step in reverse order.

@@ -15,6 +15,7 @@ copies cached per parameter version.
 
 from __future__ import annotations
 
+import math
 import os
 import weakref
 
@@ -768,6 +769,84 @@ def linear_cross_entropy_ok(x2, w, fp8: bool) -> bool:
     if fp8:
         ok = ok and M % 128 == 0 and Kd % 128 == 0 and w.shape[0] % 128 == 0
     return ok
+
+
+# --------------------------------------------------------------------------------------
+# token table: lookup with scaling, gradient by sorted tokens
+# --------------------------------------------------------------------------------------
+class _EmbeddingFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, tokens, weight, scale):
+        ctx.save_for_backward(tokens)
+        ctx.weight, ctx.scale = weight, scale
+        return _embedding_fwd(tokens, weight, scale)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, gy):
+        (tokens,) = ctx.saved_tensors
+        w = ctx.weight
+        mg = _main_grad(w)               # the buffer installed for THIS backward pass
+        if mg is not None and not _is_spread(mg) and mg.dtype == F32 and mg.is_contiguous():
+            embedding_grad(tokens, gy, w.shape[0], ctx.scale, mg.view(w.shape))
+            return None, None, None
+        return None, embedding_grad(tokens, gy, w.shape[0], ctx.scale), None
+
+
+def _embedding_fwd(tokens, weight, scale):
+    out = torch.empty(*tokens.shape, weight.shape[1], dtype=weight.dtype, device=weight.device)
+    K.token_lookup(tokens.contiguous(), weight.detach(), scale, out)
+    return out
+
+
+def embedding(tokens, weight, scale: float = 1.0):
+    """``scale * weight[tokens]``; rows move once, ids outside the table give zeros and a status code."""
+    if weight.requires_grad and torch.is_grad_enabled():
+        return _EmbeddingFn.apply(tokens, weight, scale)
+    return _embedding_fwd(tokens, weight, scale)
+
+
+def embedding_grad(tokens, grad, num_rows: int, scale: float = 1.0, out=None):
+    """Sums of the rows of ``grad`` over equal tokens: dense in ``grad``'s type, or added into the fp32 ``out``."""
+    width = grad.shape[-1]
+    g = grad.detach().reshape(tokens.numel(), width)
+    if g.stride(-1) != 1 and width != 1:
+        g = g.contiguous()
+    add = out is not None
+    if not add:
+        out = torch.empty(num_rows, width, dtype=grad.dtype, device=grad.device)
+    K.token_grad(tokens.contiguous(), g, scale, add, out)
+    if add:
+        torch.autograd.graph.increment_version(out)
+    return out
+
+
+# --------------------------------------------------------------------------------------
+# Newton-Schulz products: orthogonalised matrices and the momentum update built on them
+# --------------------------------------------------------------------------------------
+def orthogonalize(x, steps, coefficients, eps, out_dtype, pairs):
+    r, c = x.shape[-2:]
+    x3 = x.detach().reshape(math.prod(x.shape[:-2]), r, c)
+    if x3.stride(-1) != 1 and c != 1:
+        x3 = x3.contiguous()
+    out = torch.empty(x3.shape, dtype=out_dtype, device=x.device)
+    K.orthogonalize(x3, out, steps, coefficients, eps, pairs)
+    return out.view(x.shape)
+
+
+def muon_update_(params, grads, momenta, infos, scalars, *, lr, momentum, nesterov, weight_decay, steps, coefficients, eps,
+                 update_scale, beta):
+    """Matrices of one shape and type share their launches (arguments checked by the caller)."""
+    groups: dict[tuple, tuple] = {}
+    for i, p in enumerate(params):
+        lists = groups.setdefault((p.shape[-2:], p.dtype, grads[i].dtype), ([], [], [], []))
+        for to, t in zip(lists, (p, grads[i], momenta[i]) + ((infos[i],) if infos else ())):
+            to.extend(t.detach().unbind(0) if t.dim() == 3 else (t.detach(),))
+    for ((r, c), dtype, _), (ps, gs, ms, gi) in groups.items():
+        size = 0.2 * max(r, c) ** 0.5 if update_scale is None else float(update_scale)
+        K.muon_update(ps, gs, gi, ms, scalars, beta, momentum, nesterov, 1.0 - lr * weight_decay, lr * size, steps, coefficients, eps,
+                      dtype != BF16)
+    torch.autograd.graph.increment_version(params + momenta)
 
 
 # --------------------------------------------------------------------------------------

@@ -8,6 +8,9 @@ statement in ``gdnet_b200.ops.reference``. There is no other backend.
 
 from __future__ import annotations
 
+import functools
+import math
+
 import torch
 import torch.nn.functional as F
 
@@ -79,6 +82,185 @@ def sample_top_p(logits: torch.Tensor, top_p: float, generator=None) -> torch.Te
     sp = sp / sp.sum(dim=-1, keepdim=True)
     pick = torch.multinomial(sp[0], 1, generator=generator)
     return si[0, pick]
+
+
+# --------------------------------------------------------------------------------------
+# token table
+# --------------------------------------------------------------------------------------
+_TABLE_TYPES = (torch.bfloat16, torch.float16, torch.float32)
+
+
+def _check_tokens(tokens, like, what: str) -> None:
+    if tokens.dtype not in (torch.int64, torch.int32):
+        raise TypeError(f"{what}: tokens must be int64 or int32, got {tokens.dtype}")
+    if tokens.device != like.device:
+        raise ValueError(f"{what}: tokens are on {tokens.device}, the rows on {like.device}")
+
+
+def embedding(tokens, weight, scale: float = 1.0):
+    """``scale * weight[tokens]``: ``tokens`` (any shape, int64 or int32) to ``tokens.shape + (width,)`` in the type of
+    ``weight (vocab, width)`` (bf16, fp16 or fp32), multiplied in fp32 and rounded once.
+
+    Differentiable in ``weight``. On CUDA the gradient is :func:`embedding_grad`: with a ``main_grad`` installed by the
+    training engine it is added there in fp32 and autograd gets none. An id outside the table gives a row of zeros, no
+    gradient, and a bad-argument code in the kernel status word (on CPU an ``IndexError``)."""
+    if weight.dim() != 2 or weight.dtype not in _TABLE_TYPES:
+        raise TypeError(f"embedding: the table must be a bf16, fp16 or fp32 matrix, got {weight.dtype} {tuple(weight.shape)}")
+    _check_tokens(tokens, weight, "embedding")
+    if _on_gpu(weight):
+        return _cuda().embedding(tokens, weight, float(scale))
+    return ref.embedding(tokens, weight, float(scale))
+
+
+@torch.no_grad()
+def embedding_grad(tokens, grad, num_rows: int, scale: float = 1.0, out=None):
+    """Gradient of :func:`embedding`: ``(num_rows, width)``, row ``v`` is ``scale`` times the sum of the rows
+    ``grad[t]`` with ``tokens[t] == v``. ``grad`` is ``tokens.shape + (width,)``.
+
+    Without ``out`` a dense gradient in the type of ``grad`` (summed in fp32, rounded once; rows of absent ids are zero).
+    With ``out`` (fp32, contiguous) the sums are added to it, only the rows of ids that occur are touched, and ``out``
+    is returned. The rows of an id are summed in a fixed order: the same inputs give the same bits. Ids outside
+    the table are left out."""
+    if grad.dtype not in _TABLE_TYPES or grad.dim() < 1:
+        raise TypeError(f"embedding_grad: grad must be bf16, fp16 or fp32, got {grad.dtype}")
+    _check_tokens(tokens, grad, "embedding_grad")
+    if grad.shape[:-1] != tokens.shape:
+        raise ValueError(f"embedding_grad: grad {tuple(grad.shape)} does not fit tokens {tuple(tokens.shape)}")
+    num_rows = int(num_rows)
+    if num_rows < 0:
+        raise ValueError("embedding_grad: num_rows is negative")
+    if out is not None:
+        if out.dtype != torch.float32 or not out.is_contiguous() or out.device != grad.device:
+            raise ValueError("embedding_grad: out must be a contiguous fp32 tensor on the gradient's device")
+        if tuple(out.shape) != (num_rows, grad.shape[-1]):
+            raise ValueError(f"embedding_grad: out {tuple(out.shape)} is not ({num_rows}, {grad.shape[-1]})")
+    if _on_gpu(grad):
+        return _cuda().embedding_grad(tokens, grad, num_rows, float(scale), out)
+    return ref.embedding_grad(tokens, grad, num_rows, float(scale), out)
+
+
+# --------------------------------------------------------------------------------------
+# orthogonalised update of matrices
+# --------------------------------------------------------------------------------------
+NS_COEFFICIENTS = (3.4445, -4.7750, 2.0315)     # steep at zero: singular values from 1e-2 up land in about [0.7, 1.2] after five steps
+_NS_LIMIT = 3.9                                 # bound of the operand format (csrc/orthogonalize.cu)
+
+
+@functools.lru_cache(maxsize=64)
+def _ns_check(coefficients: tuple, steps: int) -> None:
+    """Refuse coefficients under which a singular value that starts in [0, 1], or a factor of the products, leaves the
+    range of the operand format."""
+    a, b, c = coefficients
+    top = 1.0
+    for _ in range(steps):
+        s = [top * i / 2048 for i in range(2049)]
+        poly = max(abs(x * (a + b * x * x + c * x**4)) for x in s)
+        factor = max(abs(b * x * x + c * x**4) for x in s)
+        if not (max(poly, factor, top * top) <= _NS_LIMIT):
+            raise ValueError(f"orthogonalize: coefficients {coefficients} let the iteration grow past {_NS_LIMIT}")
+        top = max(poly, 1e-6)
+
+
+def _ns_arguments(steps, coefficients, eps, what: str):
+    steps, eps = int(steps), float(eps)
+    coefficients = tuple(float(x) for x in coefficients)
+    if not 0 <= steps <= 100:
+        raise ValueError(f"{what}: steps must be in [0, 100], got {steps}")
+    if len(coefficients) != 3 or not all(math.isfinite(x) for x in coefficients):
+        raise ValueError(f"{what}: three finite coefficients, got {coefficients}")
+    if not (eps > 0.0 and math.isfinite(eps)):
+        raise ValueError(f"{what}: eps must be positive, got {eps}")
+    _ns_check(coefficients, steps)
+    return steps, coefficients, eps
+
+
+def _ns_pairs(dtype) -> bool:
+    """Whether the products run on pairs of fp16 values: not where the result is rounded to bf16 anyway."""
+    return dtype != torch.bfloat16
+
+
+def orthogonalize(x, steps: int = 5, coefficients=NS_COEFFICIENTS, eps: float = 1e-7, out_dtype=None):
+    """Newton-Schulz orthogonalisation of the matrices ``x (..., r, c)`` (bf16, fp16 or fp32): each is divided by its
+    Frobenius norm plus ``eps``, then its singular values go ``steps`` times through ``a s + b s^3 + c s^5`` while its singular
+    vectors stay. A matrix of zeros stays zero. Returns a new tensor in ``out_dtype`` (default: that of ``x``); a
+    bf16 result is computed from fp16 products, others as exactly as in fp32. Has no gradient."""
+    out_dtype = x.dtype if out_dtype is None else out_dtype
+    if x.dim() < 2 or x.dtype not in _TABLE_TYPES or out_dtype not in _TABLE_TYPES:
+        raise TypeError(f"orthogonalize: bf16, fp16 or fp32 matrices, got {x.dtype} {tuple(x.shape)} to {out_dtype}")
+    steps, coefficients, eps = _ns_arguments(steps, coefficients, eps, "orthogonalize")
+    if torch.is_grad_enabled() and x.requires_grad:
+        raise ValueError("orthogonalize has no gradient: detach its input")
+    if _on_gpu(x):
+        return _cuda().orthogonalize(x, steps, coefficients, eps, out_dtype, _ns_pairs(out_dtype))
+    return ref.orthogonalize(x, steps, coefficients, eps, out_dtype)
+
+
+def _overlap(written, read) -> bool:
+    """Whether a written tensor shares memory with another written or a read one (all contiguous)."""
+    spans = [(t.data_ptr(), t.data_ptr() + t.numel() * t.element_size(), 1) for t in written if t.numel()]
+    spans += [(t.data_ptr(), t.data_ptr() + t.numel() * t.element_size(), 0) for t in read if t.numel()]
+    end_any = end_written = 0
+    for lo, hi, w in sorted(spans):
+        if lo < (end_any if w else end_written):
+            return True
+        end_any = max(end_any, hi)
+        if w:
+            end_written = max(end_written, hi)
+    return False
+
+
+@torch.no_grad()
+def muon_update_(params, grads, momenta, *, lr: float, momentum: float = 0.95, nesterov: bool = True,
+                 weight_decay: float = 0.0, steps: int = 5, coefficients=NS_COEFFICIENTS, eps: float = 1e-7,
+                 update_scale: float | None = None, info_grads=None, scalars=None, beta: float = 0.0) -> None:
+    """One momentum update of matrices by orthogonalised directions, in place. For every matrix::
+
+        g <- scalars[1] * ((1 - beta * scalars[0]) * grad + beta * info_grad)      (g = grad without scalars)
+        m <- momentum * m + g;      u = g + momentum * m                           (u = m without nesterov)
+        p <- p * (1 - lr * weight_decay) - lr * update_scale * orthogonalize(u)
+
+    ``params`` (bf16, fp16 or fp32) and ``grads`` (and ``info_grads``) are lists of contiguous tensors ``(r, c)`` or banks of
+    matrices ``(n, r, c)``, ``momenta`` the same in fp32; shapes may differ from entry to entry. ``scalars`` is a
+    device tensor (projection coefficient, gradient scale) as the training engine keeps it. ``update_scale`` defaults to
+    ``0.2 sqrt(max(r, c))``, which gives the update the size of an AdamW step of the same ``lr``. No two
+    entries may share memory."""
+    params, grads, momenta = list(params), list(grads), list(momenta)
+    infos = list(info_grads) if info_grads is not None else []
+    if not (len(params) == len(grads) == len(momenta)) or (infos and len(infos) != len(params)):
+        raise ValueError("muon_update_: params, grads, momenta (and info_grads) must have the same length")
+    steps, coefficients, eps = _ns_arguments(steps, coefficients, eps, "muon_update_")
+    if infos and scalars is None:
+        raise ValueError("muon_update_: info_grads need scalars (projection coefficient, gradient scale)")
+    if not params:
+        return
+    dev = params[0].device
+    if scalars is not None and (scalars.dtype != torch.float32 or scalars.numel() < 2 or scalars.device != dev):
+        raise ValueError("muon_update_: scalars must be two fp32 values on the params' device")
+    for i, p in enumerate(params):
+        mine = [p, grads[i], momenta[i]] + ([infos[i]] if infos else [])
+        if p.dim() not in (2, 3) or any(t.shape != p.shape for t in mine):
+            raise ValueError(f"muon_update_: entry {i} needs matrices of one shape, got {[tuple(t.shape) for t in mine]}")
+        if any(t.device != dev or not t.is_contiguous() for t in mine):
+            raise ValueError(f"muon_update_: entry {i} must be contiguous and on {dev}")
+        if p.dtype not in _TABLE_TYPES or grads[i].dtype not in _TABLE_TYPES or momenta[i].dtype != torch.float32:
+            raise TypeError(f"muon_update_: entry {i} has types {[t.dtype for t in mine]}")
+        if infos and infos[i].dtype != grads[i].dtype:
+            raise TypeError(f"muon_update_: entry {i} has gradients of two types")
+    if _overlap(params + momenta, grads + infos):
+        raise ValueError("muon_update_: entries share memory")
+    hyper = dict(lr=float(lr), momentum=float(momentum), nesterov=bool(nesterov), weight_decay=float(weight_decay),
+                 steps=steps, coefficients=coefficients, eps=eps, update_scale=update_scale, beta=float(beta))
+    if dev.type == "cuda":
+        _cuda().muon_update_(params, grads, momenta, infos, scalars, **hyper)
+        return
+    for i, p in enumerate(params):
+        g = grads[i].float()
+        if scalars is not None:
+            g = (1 - beta * scalars[0]) * g + (beta * infos[i].float() if infos else 0.0)
+            g = scalars[1] * g
+        step = lr * (0.2 * math.sqrt(max(p.shape[-2:])) if update_scale is None else update_scale)
+        ref.muon_update_(p, g, momenta[i], lr=lr, momentum=momentum, nesterov=nesterov, weight_decay=weight_decay, step=step,
+                         steps=steps, coefficients=coefficients, eps=eps)
 
 
 # --------------------------------------------------------------------------------------

@@ -344,3 +344,49 @@ def projected_adamw_(p, gt, gi, m, v, *, coef, beta_proj, grad_scale, lr, beta1,
     pf = pf - (lr / bc1) * m / ((v / bc2).sqrt() + eps)
     p.copy_(pf.to(p.dtype))
     return p
+
+
+# --------------------------------------------------------------------------------------
+# token table, orthogonalised update
+# --------------------------------------------------------------------------------------
+
+def embedding(tokens: torch.Tensor, weight: torch.Tensor, scale: float = 1.0) -> torch.Tensor:
+    """``scale * weight[tokens]``, the product in fp32 and rounded once. Differentiable in ``weight``."""
+    x = F.embedding(tokens, weight)
+    return x if scale == 1.0 else (x.float() * scale).to(weight.dtype)
+
+
+def embedding_grad(tokens, grad, num_rows: int, scale: float = 1.0, out=None):
+    """Row ``v``: ``scale`` times the sum of the rows of ``grad`` whose token is ``v``, in fp32; ids outside the table
+    are left out. Added into ``out`` (fp32) or returned in ``grad``'s type."""
+    t = tokens.reshape(-1).long()
+    g = grad.reshape(t.numel(), grad.shape[-1]).float()
+    live = (t >= 0) & (t < num_rows)
+    total = torch.zeros(num_rows, g.shape[1], dtype=torch.float32, device=grad.device)
+    total.index_add_(0, t[live], g[live])
+    total = total * scale
+    return total.to(grad.dtype) if out is None else out.add_(total)
+
+
+def orthogonalize(x, steps: int, coefficients, eps: float, out_dtype) -> torch.Tensor:
+    """``steps`` times ``X <- a X + (b A + c A^2) X`` with ``A = X X^T`` (``X^T X`` from the right for tall matrices),
+    starting from ``x / (|x|_F + eps)``. ``x (..., r, c)``; fp32 arithmetic."""
+    a, b, c = coefficients
+    x = x.float()
+    x = x / (torch.linalg.vector_norm(x.double(), dim=(-2, -1), keepdim=True) + eps).float()
+    tall = x.shape[-2] > x.shape[-1]
+    x = x.mT if tall else x
+    for _ in range(steps):
+        A = x @ x.mT
+        x = a * x + (b * A + c * (A @ A)) @ x
+    return (x.mT if tall else x).to(out_dtype).contiguous()
+
+
+def muon_update_(p, g, m, *, lr, momentum, nesterov, weight_decay, step, steps, coefficients, eps):
+    """In place, one matrix: ``m <- momentum m + g``, ``u = g + momentum m`` (``m`` without nesterov),
+    ``p <- p (1 - lr weight_decay) - step orthogonalize(u)``; ``m`` fp32, ``g`` fp32."""
+    m.mul_(momentum).add_(g)
+    u = g + momentum * m if nesterov else m
+    o = orthogonalize(u, steps, coefficients, eps, torch.float32)
+    p.copy_((p.float() * (1 - lr * weight_decay) - step * o).to(p.dtype))
+    return p

@@ -89,6 +89,7 @@ def flat_layout(engine) -> list[dict]:
         out.append({
             "dtype": str(g.dtype).replace("torch.", ""),
             "numel": int(g.n),
+            "optimizer": getattr(g, "optimizer", "adamw"),
             "params": [{"name": names[id(p)], "offset": int(o), "shape": list(p.shape), "numel": int(p.numel())}
                        for p, o in zip(g.params, g.offsets)],
         })
@@ -174,11 +175,15 @@ def load_sharded(directory, engine) -> tuple[int, dict]:
     if saved_names != set(where):
         missing, extra_ = sorted(set(where) - saved_names)[:5], sorted(saved_names - set(where))[:5]
         raise CheckpointError(f"checkpoint and model disagree on the parameters (missing {missing}, unexpected {extra_})")
+    kinds = {prm["name"]: lay["optimizer"] for lay in new_layout for prm in lay["params"]}
     shapes = {prm["name"]: prm["shape"] for lay in new_layout for prm in lay["params"]}
     for lay in manifest["layout"]:
         for prm in lay["params"]:
             if list(prm["shape"]) != list(shapes[prm["name"]]):
                 raise CheckpointError(f"shape of {prm['name']} differs: checkpoint {prm['shape']}, model {shapes[prm['name']]}")
+            if lay.get("optimizer", "adamw") != kinds[prm["name"]]:
+                raise CheckpointError(f"{prm['name']} was updated by {lay.get('optimizer', 'adamw')}, the engine updates it by "
+                                      f"{kinds[prm['name']]}: its moments do not carry over")
 
     for g in engine.groups:           # ranges nothing is saved for (alignment padding) stay zero
         g.m.zero_()

@@ -25,6 +25,10 @@ One step = one forward, two backward passes (task; info + transition), then
   in this mode is computed from the reduced gradients (no rank ever holds its full local gradient);
 * N GPUs, ``comm="nccl"``: NCCL all-reduce of the flat gradients, then the 1-GPU update.
 
+``matrix_optimizer="muon"`` (one GPU, or ``comm="nccl"``) puts the large matrices of the layers into a group of their own whose
+update is ``ops.muon_update_``: projected gradient, momentum, and a step along the orthogonalised momentum. That
+group has one moment buffer instead of two; the token table, the vectors and the small heads stay on AdamW.
+
 The projection coefficient uses the sum over ranks of the *local* dot products, exactly as
 the reference does (gdnet/loss.py:228-235), and the reduced gradient is the mean over ranks
 (gdnet/loss.py:241-251).
@@ -50,8 +54,8 @@ class _Group:
 
     sharded = False
 
-    def __init__(self, params, dtype, device, world, rank, symmetric, pg):
-        self.params, self.dtype = params, dtype
+    def __init__(self, params, dtype, device, world, rank, symmetric, pg, optimizer="adamw"):
+        self.params, self.dtype, self.optimizer = params, dtype, optimizer
         offs, n = [], 0
         for p in params:
             offs.append(n)
@@ -83,7 +87,7 @@ class _Group:
                 p.data = view
         m_len = per if symmetric else self.n   # fused mode updates only this rank's shard
         self.m = torch.zeros(m_len, dtype=torch.float32, device=device)
-        self.v = torch.zeros(m_len, dtype=torch.float32, device=device)
+        self.v = torch.zeros(m_len if optimizer == "adamw" else 0, dtype=torch.float32, device=device)
         self.sums = torch.zeros(8, dtype=torch.float32, device=device)
         # NVLink multicast addresses of the three buffers: the update kernel then reduces inside the switch and
         # broadcasts with one store. Used from four ranks on (on two ranks the peer loads measured faster: 2.9 against
@@ -114,6 +118,7 @@ class _ShardedGroup:
     gradient handle is a :class:`gdnet_b200.ops.cuda.GradRef`."""
 
     sharded = True
+    optimizer = "adamw"
 
     def __init__(self, params, device, world, rank, pg, broadcast_src=None):
         from ..ops import cuda as cu
@@ -184,7 +189,7 @@ class TrainEngine(nn.Module):
                  weight_decay: float = 1e-2, precision: str = "fp8", process_group=None, sp_group=None,
                  comm: str = "fused", broadcast: bool = True, projection: str = "local",
                  share_fp8_weights: bool = False, fused_ce: bool = True, shard: str = "none",
-                 overlap_task_reduce: bool = True):
+                 overlap_task_reduce: bool = True, matrix_optimizer: str = "adamw", muon_momentum: float = 0.95):
         super().__init__()
         self.module = model
         self.precision = precision
@@ -219,23 +224,35 @@ class TrainEngine(nn.Module):
             if dev.type != "cuda" or precision != "fp8":
                 raise ValueError('shard="full" needs CUDA and precision="fp8"')
             self.comm = "scatter"           # gradients go to their owner from the weight-gradient epilogues
+        # "muon": the layer matrices move along their orthogonalised momentum, everything else stays on AdamW
+        if matrix_optimizer not in ("adamw", "muon"):
+            raise ValueError(f"unknown matrix optimizer {matrix_optimizer!r}")
+        if matrix_optimizer == "muon" and self.comm not in ("local", "nccl"):
+            raise ValueError(f'matrix_optimizer="muon" needs whole matrices and gradients on every rank: comm="nccl", not {self.comm!r}')
+        self.matrix_optimizer, self.muon_momentum = matrix_optimizer, float(muon_momentum)
         symmetric = self.comm in ("fused", "scatter")
         self._sink_ids: list[int] = []
         self._shared = None
 
         params = [p for p in model.parameters() if p.requires_grad]
         sharded_params = self._layer_matrices(model) if self.shard == "full" else []
-        taken = {id(p) for p in sharded_params}
+        muon_params = self._gate_matrices(model) if matrix_optimizer == "muon" else []
+        taken = {id(p) for p in sharded_params + muon_params}
         by_dtype: dict[torch.dtype, list] = {}
         for p in params:
             if id(p) not in taken:
                 by_dtype.setdefault(p.dtype, []).append(p)
-        for dt in by_dtype:
+        muon_by_dtype: dict[torch.dtype, list] = {}
+        for p in muon_params:
+            muon_by_dtype.setdefault(p.dtype, []).append(p)
+        for dt in (*by_dtype, *muon_by_dtype):
             if dt not in (torch.bfloat16, torch.float32):
                 raise TypeError(f"unsupported parameter dtype {dt}")
         src0 = dist.get_global_rank(self.pg, 0) if self.distributed else None
         self.groups = [
             _Group(ps, dt, dev, self.world, self.rank, symmetric, self.pg) for dt, ps in by_dtype.items()
+        ] + [
+            _Group(ps, dt, dev, self.world, self.rank, symmetric, self.pg, "muon") for dt, ps in muon_by_dtype.items()
         ]
         if sharded_params:
             self.groups.append(_ShardedGroup(sharded_params, dev, self.world, self.rank, self.pg,
@@ -321,6 +338,13 @@ class TrainEngine(nn.Module):
                 cu.remove_provider(obj)
         self._shared = None
         self.weight_stream = None
+
+    @staticmethod
+    def _gate_matrices(model):
+        """The parameters that ``matrix_optimizer="muon"`` orthogonalises the update of: the trainable matrices of every
+        GDLayer's gates."""
+        return [w for layer in getattr(model, "layers", []) for prefix in ("gf", "gb", "rf", "rb") for which in ("W1", "W2")
+                if (w := getattr(layer, f"{prefix}_{which}").weight).requires_grad and w.dim() == 2]
 
     @staticmethod
     def _layer_matrices(model):
@@ -526,7 +550,12 @@ class TrainEngine(nn.Module):
                     K.grad_dots(g.g_task, g.g_info, red)
                 self.scalars[1] = self.scalars[1] * self._clip_factor(red * self.scalars[1] ** 2, coef, beta, grad_clip)
             for g in self.groups:
-                K.projected_adamw(g.flat, g.g_task, g.g_info, g.m, g.v, self.scalars, *common)
+                if g.optimizer == "muon":
+                    ops.muon_update_([p.data for p in g.params], g.views(g.g_task), g.views(g.m), lr=self.lr,
+                                     momentum=self.muon_momentum, weight_decay=self.weight_decay,
+                                     info_grads=g.views(g.g_info), scalars=self.scalars, beta=beta)
+                else:
+                    K.projected_adamw(g.flat, g.g_task, g.g_info, g.m, g.v, self.scalars, *common)
             return
 
         # fused: reduce-scatter + projection + AdamW + all-gather over peer memory
@@ -595,6 +624,7 @@ class TrainEngine(nn.Module):
 
     def state_dict_optim(self) -> dict:
         return {"step": self.step_count, "lr": self.lr, "world": self.world, "rank": self.rank,
+                "optimizers": [g.optimizer for g in self.groups],
                 "m": [g.m.clone() for g in self.groups], "v": [g.v.clone() for g in self.groups]}
 
     def load_state_dict_optim(self, sd: dict) -> None:
@@ -602,6 +632,9 @@ class TrainEngine(nn.Module):
         own); anything else goes through ``runtime.ckpt.save_sharded`` / ``load_sharded``, which re-slice."""
         if len(sd["m"]) != len(self.groups):
             raise ValueError(f"optimizer state has {len(sd['m'])} groups, the engine {len(self.groups)}")
+        kinds = list(sd.get("optimizers", ["adamw"] * len(sd["m"])))
+        if kinds != [g.optimizer for g in self.groups]:
+            raise ValueError(f"optimizer state of {kinds} cannot be loaded into {[g.optimizer for g in self.groups]}")
         if int(sd.get("world", self.world)) != self.world or int(sd.get("rank", self.rank)) != self.rank:
             raise ValueError(f"optimizer state of rank {sd.get('rank')} / world {sd.get('world')} cannot be loaded into "
                              f"rank {self.rank} / world {self.world}: use a sharded checkpoint")

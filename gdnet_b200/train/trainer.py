@@ -240,10 +240,13 @@ def train(cfg: Config, interactive: bool = True) -> State:
         from .engine import TrainEngine
 
         runner = TrainEngine(model, lr=cfg.lr, betas=(cfg.beta1, cfg.beta2), weight_decay=cfg.weight_decay,
-                             precision=cfg.precision, sp_group=sp_group, comm=cfg.comm, shard=cfg.shard)
+                             precision=cfg.precision, sp_group=sp_group, comm=cfg.comm, shard=cfg.shard,
+                             matrix_optimizer=cfg.matrix_optimizer)
         optimizer, params = None, None
         set_lr, get_lr = runner.set_lr, (lambda: runner.lr)
     else:
+        if cfg.matrix_optimizer != "adamw":
+            raise ValueError(f"matrix_optimizer {cfg.matrix_optimizer!r} needs the training engine (CUDA, engine: true, not fp32)")
         runner = model
         if world > 1:
             from torch.nn.parallel import DistributedDataParallel as DDP
