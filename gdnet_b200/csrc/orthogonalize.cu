@@ -22,8 +22,9 @@
 
 #include <cuda_fp16.h>
 
+#include <cstring>
+
 #include "common.cuh"
-#include "launch.h"
 
 namespace gd {
 
@@ -52,34 +53,53 @@ __device__ __forceinline__ void tma_store_3d(const CUtensorMap* m, uint32_t src,
 }
 
 // ---------------------------------------------------------------------------------------
-// one product over the batch
+// all products of a call in one kernel
 // ---------------------------------------------------------------------------------------
-// D = acc_scale * P Q^T + aux_scale * aux, P (M x K), Q (N x K). Same structure as the GEMM kernels: a producer warp, an
-// MMA warp, eight epilogue warps, two accumulators in TMEM. PAIR: a pair of CTAs (two SMs) shares a 256 x 256
-// tile, each loading its half of both operands; otherwise a CTA has a 128 x 128 tile of its own (small matrices: more
-// tiles, shorter chain).
+// An item is one output tile of one product of one matrix. Items are handed out in order by a counter in memory, and an
+// item waits only for items before it: the products of a matrix follow one another, and a count of the finished
+// tiles per matrix says how far it is. So any number of resident blocks makes progress (two calls on two streams may share
+// the GPU), nothing is launched between the 3 x steps products, and the tiles of one product fill the gaps that
+// the end of another leaves. The order is: for a window of matrices, product by product, all their tiles; a window is as many
+// matrices as stay in L2 from one product to the next.
+//
+// A block: warp 0 fetches items and loads operands with bulk tensor copies into a ring of stages; warp 1 issues the MMAs into
+// two accumulators in TMEM; eight epilogue warps read the accumulator, add the linear term (its boxes are copied in
+// while the MMAs run) and send 32 x 32 boxes out with bulk stores. PAIR: a pair of CTAs on two SMs shares a
+// 256 x 256 tile, each loading its half of both operands; otherwise a CTA has a 128 x 128 tile of its own.
 constexpr int NS_BK = 64;                       // K elements per stage: one 128-byte swizzle row
 constexpr int NS_EPI_WARPS = 8;
 constexpr int NS_THREADS = 64 + NS_EPI_WARPS * 32;
 constexpr int NS_OPERAND_BYTES = 128 * 128;     // 128 rows x 64 fp16 per CTA and operand
 constexpr int NS_STAGE_BYTES = 2 * NS_OPERAND_BYTES;
-constexpr int NS_STAGES = 5;
 constexpr int NS_BOX = 32;                      // epilogue chunk: 32 x 32
-constexpr int NS_STAGING_BYTES = NS_BOX * NS_BOX * 2;                 // 2 KB
-constexpr int NS_STAGING_PER_WARP = 2 * NS_STAGING_BYTES;             // the chunk and its transpose
+constexpr int NS_BOX_BYTES = NS_BOX * NS_BOX * 2;
+constexpr int NS_SLOTS = 2;                     // chunks in flight per epilogue warp
 constexpr int NS_ACC = 2;
 constexpr int NS_SPLIT_KBLOCKS = 2;             // pairs: K blocks summed in TMEM before the sum moves to registers
+// Items on their way through a block: the loads run at most the stages (5) ahead of the MMAs, these two accumulators ahead
+// of the epilogue, and one item is fetched early; a ring of 16 is never overwritten before it is read.
+constexpr int NS_RING = 16;
+
+template <bool SPLIT>
+struct NsShape {
+  static constexpr int STAGES = SPLIT ? 3 : 5;
+  static constexpr int SLOT_BOXES = SPLIT ? 4 : 2;               // (hi, transpose | lo), with pairs (hi, lo and both transposes)
+  static constexpr int WARP_BYTES = NS_SLOTS * SLOT_BOXES * NS_BOX_BYTES;
+  static constexpr int SMEM = STAGES * NS_STAGE_BYTES + NS_EPI_WARPS * WARP_BYTES + 1024 + 1024;   // barriers; alignment
+};
 
 struct __align__(8) NsBars {
-  uint64_t full[8];
-  uint64_t empty[8];
+  uint64_t full[5];
+  uint64_t empty[5];
   uint64_t acc_full[NS_ACC];
   uint64_t acc_empty[NS_ACC];
+  uint64_t aux_full[NS_EPI_WARPS * NS_SLOTS];
+  uint64_t item_full[NS_RING];
+  int item[NS_RING];
   uint32_t tmem_base;
   int abort;
 };
-
-constexpr int NS_SMEM = NS_STAGES * NS_STAGE_BYTES + NS_EPI_WARPS * NS_STAGING_PER_WARP + (int)sizeof(NsBars) + 1024;
+static_assert(sizeof(NsBars) <= 1024, "barrier area");
 
 __device__ __forceinline__ bool ns_aborted(const NsBars* b) { return *((volatile const int*)&b->abort) != 0; }
 __device__ __forceinline__ void ns_abort(NsBars* b, Status* st, int code, int site, int detail) {
@@ -92,121 +112,150 @@ __device__ __forceinline__ bool ns_wait(uint32_t bar, uint32_t parity) {
 }
 __device__ __forceinline__ uint64_t ns_desc(uint32_t hi, uint32_t lo) { return ((uint64_t)hi << 32) | (uint64_t)lo; }
 
-// work item -> (matrix, row block, column block). Symmetric products list only column block >= row block.
-__device__ __forceinline__ void ns_tile(const NsProduct& g, int item, int& z, int& mb, int& nb) {
-  z = item / g.tiles;
-  int t = item - z * g.tiles;
-  if (!g.symmetric) {
-    nb = t / g.tiles_m;          // neighbours share a column block
-    mb = t - nb * g.tiles_m;
-    return;
+// The same wait for a word that the other CTA of the pair wrote before it arrived (acquire at cluster scope).
+__device__ __forceinline__ uint32_t ns_try_wait_cluster(uint32_t bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(bar), "r"(parity)
+      : "memory");
+  return ok;
+}
+__device__ __forceinline__ void ns_put_remote(uint32_t cluster_addr, int v) {
+  asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(cluster_addr), "r"(v) : "memory");
+}
+__device__ __forceinline__ void ns_arrive_remote(uint32_t cluster_bar) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_bar) : "memory");
+}
+
+// Item `slot_no` of this block's list, -1 at its end or when the wait ran out. Warp-collective.
+__device__ __forceinline__ int ns_next_item(NsBars* bars, int slot_no, Status* status) {
+  const uint32_t bar = smem_u32(&bars->item_full[slot_no & (NS_RING - 1)]);
+  const uint32_t parity = (slot_no / NS_RING) & 1;
+  int item = -1;
+  if ((threadIdx.x & 31) == 0) {
+    bool ok = false;
+    for (int i = 0; i < 256 && !ok; ++i) ok = ns_try_wait_cluster(bar, parity);
+    if (!ok) {
+      const uint64_t t0 = globaltimer_ns();
+      while (!(ok = ns_try_wait_cluster(bar, parity))) {
+        __nanosleep(32);
+        if (ns_aborted(bars)) break;
+        if (globaltimer_ns() - t0 > GD_WAIT_BUDGET_NS) {
+          ns_abort(bars, status, STATUS_TIMEOUT_SMEM_FULL, 87, slot_no);
+          break;
+        }
+      }
+    }
+    if (ok) item = *((volatile int*)&bars->item[slot_no & (NS_RING - 1)]);
   }
-  // column block nb holds the nb + 1 tiles t = nb (nb + 1) / 2 ... (blocks per side are few: count up)
-  nb = 0;
-  while (t > nb) { t -= nb + 1; ++nb; }
-  mb = t;
+  return __shfl_sync(0xffffffffu, item, 0);
+}
+
+struct NsItem {
+  int step, phase, z, mb, nb;        // phase 0: A, 1: B, 2: X
+  uint32_t need;                     // finished tiles of matrix z that this one reads (in epilogue warps)
+};
+
+__device__ __forceinline__ NsItem ns_decode(const NsPlan& g, int item, uint32_t warps_per_tile) {
+  NsItem t;
+  const int per_step = 2 * g.tiles_sym + g.tiles_x;
+  const int per_window = g.window * g.steps * per_step;
+  const int win = item / per_window;
+  int r = item - win * per_window;
+  const int z0 = win * g.window, count = min(g.window, g.batch - z0);
+  t.step = r / (count * per_step);
+  r -= t.step * count * per_step;
+  const int sym = count * g.tiles_sym;
+  int tiles = g.tiles_sym;
+  t.phase = 0;
+  if (r >= 2 * sym) { t.phase = 2; r -= 2 * sym; tiles = g.tiles_x; }
+  else if (r >= sym) { t.phase = 1; r -= sym; }
+  t.z = r / tiles;
+  r -= t.z * tiles;
+  t.z += z0;
+  t.need = (uint32_t)(t.step * per_step + t.phase * g.tiles_sym) * warps_per_tile;
+  if (t.phase == 2) {
+    t.nb = r / g.tiles_xm;           // neighbours share a column block
+    t.mb = r - t.nb * g.tiles_xm;
+  } else {
+    int nb = 0;                      // column block nb holds the nb + 1 tiles on and above the diagonal
+    while (r > nb) { r -= nb + 1; ++nb; }
+    t.nb = nb;
+    t.mb = r;
+  }
+  return t;
 }
 
 // 16-byte piece `slot` (0..3) of row `row` of a 32 x 64-byte box in the 64-byte swizzle order of the bulk copies
 __device__ __forceinline__ uint32_t ns_box_off(int row, int slot) {
   return (uint32_t)(row * 64 + ((slot ^ ((row >> 1) & 3)) << 4));
 }
-
 __device__ __forceinline__ uint32_t pack_half2(float lo, float hi) {
   const __half2 h = __floats2half2_rn(lo, hi);
   return *reinterpret_cast<const uint32_t*>(&h);
 }
-
-// The staging boxes may still be the source of a bulk store of this warp: wait until it has been read. Warp-collective.
-__device__ __forceinline__ void stage_drain() {
-  if (elect_one()) bulk_wait_read_all();
-  __syncwarp();
-}
-
-// One 32 x 32 chunk (this lane's row in w) to the box at column x, row y of matrix z. Warp-collective.
-__device__ __forceinline__ void ns_put_box(uint8_t* stage, int lane, const uint32_t (&w)[16], const CUtensorMap* map, int x,
-                                           int y, int z) {
-#pragma unroll
-  for (int q = 0; q < 4; ++q)
-    *reinterpret_cast<uint4*>(stage + ns_box_off(lane, q)) = make_uint4(w[4 * q], w[4 * q + 1], w[4 * q + 2], w[4 * q + 3]);
-  fence_proxy_async_smem();
-  __syncwarp();
-  if (elect_one()) {
-    tma_store_3d(map, smem_u32(stage), x, y, z);
-    bulk_commit_group();
-  }
-  __syncwarp();
-}
-
-// The transpose of the same chunk to column x, row y: column j of the chunk becomes row j of the box.
-__device__ __forceinline__ void ns_put_box_t(uint8_t* stage, int lane, const uint32_t (&w)[16], const CUtensorMap* map, int x,
-                                             int y, int z) {
-#pragma unroll
-  for (int j = 0; j < 16; ++j) {
-    *reinterpret_cast<uint16_t*>(stage + ns_box_off(2 * j, lane >> 3) + (lane & 7) * 2) = (uint16_t)(w[j] & 0xffffu);
-    *reinterpret_cast<uint16_t*>(stage + ns_box_off(2 * j + 1, lane >> 3) + (lane & 7) * 2) = (uint16_t)(w[j] >> 16);
-  }
-  fence_proxy_async_smem();
-  __syncwarp();
-  if (elect_one()) {
-    tma_store_3d(map, smem_u32(stage), x, y, z);
-    bulk_commit_group();
-  }
-  __syncwarp();
-}
-
-// rows [0, rows_valid) x 32 fp16 of a row-major matrix -> this lane's row (coalesced: 8 rows x 64 bytes at a time)
-__device__ __forceinline__ void ns_get_rows(uint8_t* stage, int lane, uint32_t (&w)[16], const __half* base, int64_t ld,
-                                            int rows_valid) {
-  const int r_in = lane >> 2, slot = lane & 3;
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const int row = r_in + 8 * j;
-    uint4 u = make_uint4(0, 0, 0, 0);
-    if (row < rows_valid) u = *reinterpret_cast<const uint4*>(base + (int64_t)row * ld + slot * 8);
-    *reinterpret_cast<uint4*>(stage + ns_box_off(row, slot)) = u;
-  }
-  __syncwarp();
-#pragma unroll
-  for (int q = 0; q < 4; ++q) {
-    const uint4 u = *reinterpret_cast<const uint4*>(stage + ns_box_off(lane, q));
-    w[4 * q] = u.x; w[4 * q + 1] = u.y; w[4 * q + 2] = u.z; w[4 * q + 3] = u.w;
-  }
-  __syncwarp();
-}
-
 __device__ __forceinline__ float2 unpack_half2(uint32_t u) {
   return __half22float2(*reinterpret_cast<const __half2*>(&u));
 }
 
+// This lane's row of a box, in registers <-> shared memory
+__device__ __forceinline__ void ns_write_row(uint8_t* box, int lane, const uint32_t (&w)[16]) {
+#pragma unroll
+  for (int q = 0; q < 4; ++q)
+    *reinterpret_cast<uint4*>(box + ns_box_off(lane, q)) = make_uint4(w[4 * q], w[4 * q + 1], w[4 * q + 2], w[4 * q + 3]);
+}
+__device__ __forceinline__ void ns_read_row(const uint8_t* box, int lane, uint32_t (&w)[16]) {
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    const uint4 u = *reinterpret_cast<const uint4*>(box + ns_box_off(lane, q));
+    w[4 * q] = u.x; w[4 * q + 1] = u.y; w[4 * q + 2] = u.z; w[4 * q + 3] = u.w;
+  }
+}
+// The transpose of the box: column j becomes row j. Neighbouring lanes exchange halves so that a store moves two rows' values.
+__device__ __forceinline__ void ns_write_transposed(uint8_t* box, int lane, const uint32_t (&w)[16]) {
+#pragma unroll
+  for (int t = 0; t < 16; ++t) {
+    const uint32_t other = __shfl_xor_sync(0xffffffffu, w[t], 1);
+    const uint32_t v = (lane & 1) ? __byte_perm(other, w[t], 0x7632) : __byte_perm(w[t], other, 0x5410);
+    *reinterpret_cast<uint32_t*>(box + ns_box_off(2 * t + (lane & 1), lane >> 3) + ((lane >> 1) & 3) * 4) = v;
+  }
+}
+
 template <bool PAIR, bool SPLIT>
-__device__ __forceinline__ void ns_product_body(const NsMaps& maps, const NsProduct& g, Status* status) {
-  constexpr int TILE_M = PAIR ? 256 : 128, TILE_N = PAIR ? 256 : 128;
-  constexpr int ACC_COLS = TILE_N;
-  constexpr int CHUNKS = TILE_N / 64;            // 32-column chunks per epilogue warp (two warps share a lane quarter)
+__device__ __forceinline__ void ns_chain_body(const NsPlan& g, Status* status) {
+  constexpr int TILE = PAIR ? 256 : 128;
+  constexpr int CHUNKS = TILE / 64;              // 32-column chunks per epilogue warp (two warps share a lane quarter)
+  constexpr int SEGS = SPLIT ? 3 : 1;
+  constexpr int STAGES = NsShape<SPLIT>::STAGES, SLOT_BOXES = NsShape<SPLIT>::SLOT_BOXES;
+  constexpr uint32_t WARPS_PER_TILE = (PAIR ? 2 : 1) * NS_EPI_WARPS;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint8_t* staging = smem + NS_STAGES * NS_STAGE_BYTES;
-  NsBars* bars = reinterpret_cast<NsBars*>(staging + NS_EPI_WARPS * NS_STAGING_PER_WARP);
+  uint8_t* boxes = smem + STAGES * NS_STAGE_BYTES;
+  NsBars* bars = reinterpret_cast<NsBars*>(boxes + NS_EPI_WARPS * NsShape<SPLIT>::WARP_BYTES);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = PAIR ? cluster_ctarank() : 0;
-  const int unit = PAIR ? (int)(blockIdx.x >> 1) : (int)blockIdx.x, units = PAIR ? (int)(gridDim.x >> 1) : (int)gridDim.x;
 
   if (warp == 0 && lane == 0) {
-    for (int s = 0; s < NS_STAGES; ++s) {
+    for (int s = 0; s < STAGES; ++s) {
       mbar_init(smem_u32(&bars->full[s]), 1);
       mbar_init(smem_u32(&bars->empty[s]), 1);
     }
     for (int a = 0; a < NS_ACC; ++a) {
       mbar_init(smem_u32(&bars->acc_full[a]), 1);
-      mbar_init(smem_u32(&bars->acc_empty[a]), (PAIR ? 2 : 1) * NS_EPI_WARPS);
+      mbar_init(smem_u32(&bars->acc_empty[a]), WARPS_PER_TILE);
     }
+    for (int a = 0; a < NS_EPI_WARPS * NS_SLOTS; ++a) mbar_init(smem_u32(&bars->aux_full[a]), 1);
+    for (int a = 0; a < NS_RING; ++a) mbar_init(smem_u32(&bars->item_full[a]), 1);
     bars->abort = 0;
     fence_barrier_init();
   }
   if (warp == 1) {
-    if (PAIR) { tmem_alloc_pair(smem_u32(&bars->tmem_base), NS_ACC * ACC_COLS); tmem_relinquish_pair(); }
-    else { tmem_alloc(smem_u32(&bars->tmem_base), NS_ACC * ACC_COLS); tmem_relinquish(); }
+    if (PAIR) { tmem_alloc_pair(smem_u32(&bars->tmem_base), NS_ACC * TILE); tmem_relinquish_pair(); }
+    else { tmem_alloc(smem_u32(&bars->tmem_base), NS_ACC * TILE); tmem_relinquish(); }
   }
   tc_fence_before_sync();
   __syncthreads();
@@ -215,29 +264,58 @@ __device__ __forceinline__ void ns_product_body(const NsMaps& maps, const NsProd
   pdl_enter();
   const uint32_t tmem_base = bars->tmem_base;
 
-  const int n_work = g.batch * g.tiles;
-  const int kblocks = (g.K + NS_BK - 1) / NS_BK;
-  constexpr int SEGS = SPLIT ? 3 : 1;
-  // K blocks that one accumulator in TMEM takes: all of them, or, with pairs, few enough for the sum to stay as exact as fp32
-  const int per_acc = SPLIT ? NS_SPLIT_KBLOCKS : kblocks;
-  const int n_acc = (kblocks * SEGS + per_acc - 1) / per_acc;
+  const int kb_x = (g.wide + NS_BK - 1) / NS_BK, kb_k = (g.k + NS_BK - 1) / NS_BK;   // K blocks of product A; of B and X
   const uint32_t smem0 = smem_u32(smem);
   const uint32_t full0 = smem_u32(&bars->full[0]), empty0 = smem_u32(&bars->empty[0]);
   const uint32_t afull0 = smem_u32(&bars->acc_full[0]), aempty0 = smem_u32(&bars->acc_empty[0]);
 
   if (warp == 0) {
     const uint32_t full_lead0 = PAIR ? map_to_cta(full0, 0) : full0;
-    int s = 0;
+    const uint32_t peer_item0 = PAIR ? map_to_cta(smem_u32(&bars->item[0]), rank ^ 1) : 0;
+    const uint32_t peer_bar0 = PAIR ? map_to_cta(smem_u32(&bars->item_full[0]), rank ^ 1) : 0;
+    int s = 0, ahead = 0;
     uint32_t ph = 0;
     bool ok = true;
-    for (int work = unit; work < n_work && ok; work += units) {
-      int z, mb, nb;
-      ns_tile(g, work, z, mb, nb);
-      const int m0 = mb * TILE_M + (int)rank * 128, n0 = nb * TILE_N + (int)rank * 128;
+    if (rank == 0 && lane == 0) ahead = (int)atomicAdd(g.next_item, 1u);
+    for (int it = 0; ok; ++it) {
+      int item;
+      if (rank == 0) {
+        item = __shfl_sync(0xffffffffu, ahead, 0);
+        if (item >= g.items || ns_aborted(bars)) item = -1;
+        if (lane == 0) {
+          const int slot = it & (NS_RING - 1);
+          *((volatile int*)&bars->item[slot]) = item;
+          mbar_arrive(smem_u32(&bars->item_full[slot]));
+          if (PAIR) {
+            ns_put_remote(peer_item0 + 4 * slot, item);
+            ns_arrive_remote(peer_bar0 + 8 * slot);
+          }
+          if (item >= 0) ahead = (int)atomicAdd(g.next_item, 1u);      // needed one item later
+        }
+        __syncwarp();
+      } else {
+        item = ns_next_item(bars, it, status);
+      }
+      if (item < 0) break;
+      const NsItem t = ns_decode(g, item, WARPS_PER_TILE);
+      uint32_t ready = 1;
+      if (lane == 0 && t.need != 0) ready = wait_flag_ge_gpu(g.done + t.z, t.need, GD_WAIT_BUDGET_NS);
+      if (!__shfl_sync(0xffffffffu, ready, 0)) {
+        if (lane == 0) ns_abort(bars, status, STATUS_TIMEOUT_PEER_FLAG, 84, t.z);
+        break;
+      }
+      fence_proxy_async_global();      // what other blocks wrote before they counted up is read by bulk copies below
+      const int cur = t.step & 1;
+      const int m0 = t.mb * TILE + (int)rank * 128, n0 = t.nb * TILE + (int)rank * 128;
+      const bool p_mn = t.phase == 0 && g.tall, q_mn = t.phase == 0 ? g.tall : (t.phase == 2 && !g.tall);
+      const int kblocks = t.phase == 0 ? kb_x : kb_k;
       for (int seg = 0; seg < SEGS && ok; ++seg) {
         // hi lo, lo hi, hi hi: the small partial products first
-        const CUtensorMap* ma = (SPLIT && seg == 1) ? &maps.p_lo : &maps.p_hi;
-        const CUtensorMap* mq = (SPLIT && seg == 0) ? &maps.q_lo : &maps.q_hi;
+        const int p_lo = (SPLIT && seg == 1) ? 1 : 0, q_lo = (SPLIT && seg == 0) ? 1 : 0;
+        const CUtensorMap* mp = t.phase == 0 ? &g.x_gram[cur][p_lo]
+                                             : (t.phase == 1 ? &g.a_load[p_lo] : (g.tall ? &g.x_apply[cur][p_lo] : &g.b_load[p_lo]));
+        const CUtensorMap* mq = t.phase == 0 ? &g.x_gram[cur][q_lo]
+                                             : (t.phase == 1 ? &g.a_load[q_lo] : (g.tall ? &g.b_load[q_lo] : &g.x_apply[cur][q_lo]));
         for (int kb = 0, kx = 0; kb < kblocks; ++kb, kx += NS_BK) {
           if (!__all_sync(0xffffffffu, ns_wait(empty0 + 8 * s, ph ^ 1))) {
             if (lane == 0) ns_abort(bars, status, STATUS_TIMEOUT_SMEM_EMPTY, 80, s);
@@ -245,51 +323,57 @@ __device__ __forceinline__ void ns_product_body(const NsMaps& maps, const NsProd
             break;
           }
           const uint32_t full = full_lead0 + 8 * s;
-          const uint32_t a_dst = smem0 + s * NS_STAGE_BYTES, q_dst = a_dst + NS_OPERAND_BYTES;
+          const uint32_t p_dst = smem0 + s * NS_STAGE_BYTES, q_dst = p_dst + NS_OPERAND_BYTES;
           if (elect_one()) {
             if (!PAIR || rank == 0) mbar_arrive_expect_tx(full0 + 8 * s, (PAIR ? 2 : 1) * NS_STAGE_BYTES);
             auto load = [&](uint32_t dst, const CUtensorMap* m, int x, int y) {
-              if (PAIR) tma_load_3d_pair(dst, m, full, x, y, z);
-              else tma_load_3d(dst, m, full, x, y, z);
+              if (PAIR) tma_load_3d_pair(dst, m, full, x, y, t.z);
+              else tma_load_3d(dst, m, full, x, y, t.z);
             };
-            if (!g.p_mn) load(a_dst, ma, kx, m0);
+            if (!p_mn) load(p_dst, mp, kx, m0);
             else {
 #pragma unroll
-              for (int i = 0; i < 2; ++i) load(a_dst + i * (NS_BK * 128), ma, m0 + i * 64, kx);
+              for (int i = 0; i < 2; ++i) load(p_dst + i * (NS_BK * 128), mp, m0 + i * 64, kx);
             }
-            if (!g.q_mn) load(q_dst, mq, kx, n0);
+            if (!q_mn) load(q_dst, mq, kx, n0);
             else {
 #pragma unroll
               for (int i = 0; i < 2; ++i) load(q_dst + i * (NS_BK * 128), mq, n0 + i * 64, kx);
             }
           }
           __syncwarp();
-          if (++s == NS_STAGES) { s = 0; ph ^= 1; }
+          if (++s == STAGES) { s = 0; ph ^= 1; }
         }
       }
-      if (ns_aborted(bars)) break;
     }
   } else if (warp == 1) {
     if (rank == 0) {
-      const uint32_t idesc = make_instr_desc(0, 0, g.p_mn ? 1 : 0, g.q_mn ? 1 : 0, TILE_M, TILE_N);
-      const uint32_t p_lbo = g.p_mn ? NS_BK * 128 : 16, q_lbo = g.q_mn ? NS_BK * 128 : 16;
-      const uint32_t p_step = g.p_mn ? (16 * 128) >> 4 : 2, q_step = g.q_mn ? (16 * 128) >> 4 : 2;
-      const uint64_t p_tmpl = make_smem_desc(smem0, p_lbo, 1024), q_tmpl = make_smem_desc(smem0 + NS_OPERAND_BYTES, q_lbo, 1024);
-      const uint32_t p_hi = (uint32_t)(p_tmpl >> 32), p_lo0 = (uint32_t)p_tmpl;
-      const uint32_t q_hi = (uint32_t)(q_tmpl >> 32), q_lo0 = (uint32_t)q_tmpl;
       int s = 0, acc = 0;
       uint32_t ph = 0, acc_ph = 0;
       bool ok = true;
-      for (int work = unit; work < n_work && ok; work += units) {
-        for (int part = 0; part < n_acc && ok; ++part) {
+      for (int it = 0; ok; ++it) {
+        const int item = ns_next_item(bars, it, status);
+        if (item < 0) break;
+        const NsItem t = ns_decode(g, item, WARPS_PER_TILE);
+        const bool p_mn = t.phase == 0 && g.tall, q_mn = t.phase == 0 ? g.tall : (t.phase == 2 && !g.tall);
+        const uint32_t idesc = make_instr_desc(0, 0, p_mn ? 1 : 0, q_mn ? 1 : 0, TILE, TILE);
+        const uint32_t p_step = p_mn ? (16 * 128) >> 4 : 2, q_step = q_mn ? (16 * 128) >> 4 : 2;
+        const uint64_t p_tmpl = make_smem_desc(smem0, p_mn ? NS_BK * 128 : 16, 1024);
+        const uint64_t q_tmpl = make_smem_desc(smem0 + NS_OPERAND_BYTES, q_mn ? NS_BK * 128 : 16, 1024);
+        const uint32_t p_hi = (uint32_t)(p_tmpl >> 32), p_lo0 = (uint32_t)p_tmpl;
+        const uint32_t q_hi = (uint32_t)(q_tmpl >> 32), q_lo0 = (uint32_t)q_tmpl;
+        const int blocks = (t.phase == 0 ? kb_x : kb_k) * SEGS;
+        // K blocks that one accumulator takes: all of them, or, with pairs, few enough for the sum to stay as exact as fp32
+        const int per_acc = SPLIT ? NS_SPLIT_KBLOCKS : blocks;
+        for (int b0 = 0; b0 < blocks && ok; b0 += per_acc) {
           if (!__all_sync(0xffffffffu, ns_wait(aempty0 + 8 * acc, acc_ph ^ 1))) {
             if (lane == 0) ns_abort(bars, status, STATUS_TIMEOUT_TMEM_EMPTY, 81, acc);
             ok = false;
             break;
           }
           tc_fence_after_sync();
-          const uint32_t d_tmem = tmem_base + acc * ACC_COLS;
-          const int count = min(per_acc, kblocks * SEGS - part * per_acc);
+          const uint32_t d_tmem = tmem_base + acc * TILE;
+          const int count = min(per_acc, blocks - b0);
           uint32_t accumulate = 0;
           for (int i = 0; i < count; ++i) {
             if (!__all_sync(0xffffffffu, ns_wait(full0 + 8 * s, ph))) {
@@ -312,7 +396,7 @@ __device__ __forceinline__ void ns_product_body(const NsMaps& maps, const NsProd
             }
             __syncwarp();
             accumulate = 1;
-            if (++s == NS_STAGES) { s = 0; ph ^= 1; }
+            if (++s == STAGES) { s = 0; ph ^= 1; }
           }
           if (!ok || ns_aborted(bars)) { ok = false; break; }
           if (elect_one()) {
@@ -326,19 +410,52 @@ __device__ __forceinline__ void ns_product_body(const NsMaps& maps, const NsProd
     }
   } else {
     const int ew = warp - 2;
-    uint8_t* box = staging + ew * NS_STAGING_PER_WARP;
-    uint8_t* box_t = box + NS_STAGING_BYTES;
+    uint8_t* my_boxes = boxes + ew * NsShape<SPLIT>::WARP_BYTES;
+    const uint32_t aux_bar0 = smem_u32(&bars->aux_full[ew * NS_SLOTS]);
     const int quarter = warp & 3, half = ew >> 2;
     const uint32_t aempty_lead0 = PAIR ? map_to_cta(aempty0, 0) : aempty0;
     int acc = 0;
-    uint32_t acc_ph = 0;
-    for (int work = unit; work < n_work && !ns_aborted(bars); work += units) {
-      int z, mb, nb;
-      ns_tile(g, work, z, mb, nb);
-      const int m_warp = mb * TILE_M + (int)rank * 128 + quarter * 32;
-      const int n_half = nb * TILE_N + half * (TILE_N / 2);
-      const bool mirror = g.symmetric && mb != nb;
-      const int rows_valid = min(32, g.M - m_warp);
+    uint32_t acc_ph = 0, aux_ph = 0;             // aux_ph: bit s = phase of slot s
+    bool ok = true;
+    for (int it = 0; ok; ++it) {
+      const int item = ns_next_item(bars, it, status);
+      if (item < 0) break;
+      const NsItem t = ns_decode(g, item, WARPS_PER_TILE);
+      const int cur = t.step & 1;
+      const int M = t.phase == 2 ? g.rows : g.k, N = t.phase == 2 ? g.cols : g.k;
+      const int m_warp = t.mb * TILE + (int)rank * 128 + quarter * 32;
+      const int n_half = t.nb * TILE + half * (TILE / 2);
+      const bool mirror = t.phase != 2 && t.mb != t.nb;
+      const CUtensorMap* out = t.phase == 0 ? g.a_box : (t.phase == 1 ? g.b_box : g.x_box[cur ^ 1]);
+      const CUtensorMap* aux = t.phase == 1 ? g.a_box : g.x_box[cur];
+      const bool aux_lo = SPLIT || t.phase == 2, store_lo = aux_lo;
+      const float aux_scale = t.phase == 1 ? g.b : g.a, acc_scale = (t.phase == 1 ? g.c : 1.0f) * NS_UNSCALE;
+      // chunks that hold anything of the matrix: the others are not read, computed or stored
+      const int chunks = m_warp < M ? max(0, min(CHUNKS, (N - n_half + 31) / 32)) : 0;
+
+      // the slot is free once its last bulk store has been read; then the linear term's boxes land in it
+      auto aux_request = [&](int c) {
+        if (elect_one()) {
+          bulk_wait_read_all();
+          const int sl = c & (NS_SLOTS - 1);
+          const uint32_t bar = aux_bar0 + 8 * sl, dst = smem_u32(my_boxes) + sl * (SLOT_BOXES * NS_BOX_BYTES);
+          mbar_arrive_expect_tx(bar, (aux_lo ? 2 : 1) * NS_BOX_BYTES);
+          tma_load_3d(dst, &aux[0], bar, n_half + c * 32, m_warp, t.z);
+          if (aux_lo) tma_load_3d(dst + NS_BOX_BYTES, &aux[1], bar, n_half + c * 32, m_warp, t.z);
+        }
+        __syncwarp();
+      };
+      if (t.phase != 0 && chunks > 0) {
+        uint32_t ready = 1;
+        if (lane == 0) ready = wait_flag_ge_gpu(g.done + t.z, t.need, GD_WAIT_BUDGET_NS);
+        if (!__shfl_sync(0xffffffffu, ready, 0)) {
+          ns_abort(bars, status, STATUS_TIMEOUT_PEER_FLAG, 85, t.z);
+          break;
+        }
+        fence_proxy_async_global();
+        for (int c = 0; c < min(chunks, NS_SLOTS); ++c) aux_request(c);
+      }
+
       auto acc_wait = [&]() -> bool {
         if (mbar_wait_warp(afull0 + 8 * acc, acc_ph)) {
           tc_fence_after_sync();
@@ -354,8 +471,9 @@ __device__ __forceinline__ void ns_product_body(const NsMaps& maps, const NsProd
           if (PAIR) mbar_arrive_cluster(aempty_lead0 + 8 * acc);
           else mbar_arrive(aempty0 + 8 * acc);
         }
+        if (++acc == NS_ACC) { acc = 0; acc_ph ^= 1; }
       };
-      auto acc_row = [&]() { return tmem_base + ((uint32_t)(quarter * 32) << 16) + acc * ACC_COLS + half * (TILE_N / 2); };
+      auto acc_row = [&]() { return tmem_base + ((uint32_t)(quarter * 32) << 16) + acc * TILE + half * (TILE / 2); };
       // Pairs: the tensor core cuts a running sum where fp32 rounds it, an error of one sign that grows with the number of
       // additions, so every few K blocks the sum moves to registers and is continued there.
       float sum[SPLIT ? CHUNKS : 1][32];
@@ -364,8 +482,8 @@ __device__ __forceinline__ void ns_product_body(const NsMaps& maps, const NsProd
         for (int c = 0; c < CHUNKS; ++c)
 #pragma unroll
           for (int j = 0; j < 32; ++j) sum[SPLIT ? c : 0][j] = 0.0f;
-        bool ok = true;
-        for (int part = 0; part < n_acc; ++part) {
+        const int blocks = (t.phase == 0 ? kb_x : kb_k) * SEGS;
+        for (int b0 = 0; b0 < blocks && ok; b0 += NS_SPLIT_KBLOCKS) {
           if (!(ok = acc_wait())) break;
 #pragma unroll
           for (int c = 0; c < CHUNKS; ++c) {
@@ -376,70 +494,108 @@ __device__ __forceinline__ void ns_product_body(const NsMaps& maps, const NsProd
             for (int j = 0; j < 32; ++j) sum[SPLIT ? c : 0][j] += __uint_as_float(raw[j]);
           }
           acc_release();
-          if (++acc == NS_ACC) { acc = 0; acc_ph ^= 1; }
         }
         if (!ok) break;
-      } else if (!acc_wait()) {
-        break;
+      } else {
+        if (!(ok = acc_wait())) break;
+        if (chunks == 0) acc_release();
       }
-#pragma unroll(SPLIT ? CHUNKS : 1)
-      for (int c = 0; c < CHUNKS; ++c) {
-        uint32_t raw[32];
-        if (!SPLIT) tmem_ld_32x32(acc_row() + c * 32, raw);
-        const int n0 = n_half + c * 32;
-        const bool live = m_warp < g.M && n0 < g.N;      // warp-uniform
-        float aux[32];
-        if (live && g.aux_hi != nullptr) {
-          const int64_t off = (int64_t)z * g.aux_stride + (int64_t)m_warp * g.aux_ld + n0;
-          uint32_t w[16];
-          stage_drain();
-          ns_get_rows(box, lane, w, g.aux_hi + off, g.aux_ld, rows_valid);
-#pragma unroll
-          for (int t = 0; t < 16; ++t) {
-            const float2 f = unpack_half2(w[t]);
-            aux[2 * t] = f.x; aux[2 * t + 1] = f.y;
+      auto do_chunk = [&](int c, uint32_t (&raw)[32]) {
+        const int sl = c & (NS_SLOTS - 1);
+        uint8_t* slot = my_boxes + sl * (SLOT_BOXES * NS_BOX_BYTES);
+        float aux_v[32];
+        if (t.phase != 0) {
+          if (!mbar_wait_warp(aux_bar0 + 8 * sl, (aux_ph >> sl) & 1)) {
+            ns_abort(bars, status, STATUS_TIMEOUT_SMEM_FULL, 86, ew);
+            ok = false;
+            return;
           }
-          if (g.aux_lo != nullptr) {
-            ns_get_rows(box, lane, w, g.aux_lo + off, g.aux_ld, rows_valid);
+          aux_ph ^= 1u << sl;
+          uint32_t w[16];
+          ns_read_row(slot, lane, w);
 #pragma unroll
-            for (int t = 0; t < 16; ++t) {
-              const float2 f = unpack_half2(w[t]);
-              aux[2 * t] += f.x; aux[2 * t + 1] += f.y;
+          for (int i = 0; i < 16; ++i) {
+            const float2 f = unpack_half2(w[i]);
+            aux_v[2 * i] = f.x; aux_v[2 * i + 1] = f.y;
+          }
+          if (aux_lo) {
+            ns_read_row(slot + NS_BOX_BYTES, lane, w);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              const float2 f = unpack_half2(w[i]);
+              aux_v[2 * i] += f.x; aux_v[2 * i + 1] += f.y;
             }
           }
         } else {
 #pragma unroll
-          for (int j = 0; j < 32; ++j) aux[j] = 0.0f;
+          for (int j = 0; j < 32; ++j) aux_v[j] = 0.0f;
+          if (elect_one()) bulk_wait_read_but_one();      // the store that used this slot two chunks ago
+          __syncwarp();
         }
-        if (SPLIT) {
-#pragma unroll
-          for (int j = 0; j < 32; ++j) raw[j] = __float_as_uint(sum[SPLIT ? c : 0][j]);
-        } else {
+        if (!SPLIT) {
           tmem_ld_wait();
-          if (c == CHUNKS - 1) acc_release();
+          if (c == chunks - 1) acc_release();
         }
-        if (!live) continue;
         uint32_t hi[16], lo[16];
 #pragma unroll
-        for (int t = 0; t < 16; ++t) {
-          const float v0 = fmaf(g.aux_scale, aux[2 * t], g.acc_scale * __uint_as_float(raw[2 * t]));
-          const float v1 = fmaf(g.aux_scale, aux[2 * t + 1], g.acc_scale * __uint_as_float(raw[2 * t + 1]));
-          hi[t] = pack_half2(v0, v1);
-          const float2 h = unpack_half2(hi[t]);
-          lo[t] = pack_half2(v0 - h.x, v1 - h.y);
+        for (int i = 0; i < 16; ++i) {
+          const float v0 = fmaf(aux_scale, aux_v[2 * i], acc_scale * __uint_as_float(raw[2 * i]));
+          const float v1 = fmaf(aux_scale, aux_v[2 * i + 1], acc_scale * __uint_as_float(raw[2 * i + 1]));
+          hi[i] = pack_half2(v0, v1);
+          const float2 h = unpack_half2(hi[i]);
+          lo[i] = pack_half2(v0 - h.x, v1 - h.y);
         }
-        stage_drain();
-        ns_put_box(box, lane, hi, &maps.out_hi, n0, m_warp, z);
-        if (mirror) ns_put_box_t(box_t, lane, hi, &maps.out_hi, m_warp, n0, z);
-        if (g.store_lo) {
-          stage_drain();
-          ns_put_box(box, lane, lo, &maps.out_lo, n0, m_warp, z);
-          if (mirror) ns_put_box_t(box_t, lane, lo, &maps.out_lo, m_warp, n0, z);
+        __syncwarp();      // every lane has read its rows of the slot
+        uint8_t* box_t = slot + (SPLIT ? 2 : 1) * NS_BOX_BYTES;
+        ns_write_row(slot, lane, hi);
+        if (store_lo) ns_write_row(slot + NS_BOX_BYTES, lane, lo);
+        if (mirror) {
+          ns_write_transposed(box_t, lane, hi);
+          if (SPLIT) ns_write_transposed(box_t + NS_BOX_BYTES, lane, lo);
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (elect_one()) {
+          const int n0 = n_half + c * 32;
+          tma_store_3d(&out[0], smem_u32(slot), n0, m_warp, t.z);
+          if (store_lo) tma_store_3d(&out[1], smem_u32(slot + NS_BOX_BYTES), n0, m_warp, t.z);
+          if (mirror) {
+            tma_store_3d(&out[0], smem_u32(box_t), m_warp, n0, t.z);
+            if (SPLIT) tma_store_3d(&out[1], smem_u32(box_t + NS_BOX_BYTES), m_warp, n0, t.z);
+          }
+          bulk_commit_group();
+        }
+        __syncwarp();
+        if (t.phase != 0 && c + NS_SLOTS < chunks) aux_request(c + NS_SLOTS);
+      };
+      if constexpr (SPLIT) {
+#pragma unroll
+        for (int c = 0; c < CHUNKS; ++c) {
+          if (c >= chunks || !ok) continue;
+          uint32_t raw[32];
+#pragma unroll
+          for (int j = 0; j < 32; ++j) raw[j] = __float_as_uint(sum[c][j]);
+          do_chunk(c, raw);
+        }
+      } else {
+#pragma unroll 1
+        for (int c = 0; c < chunks && ok; ++c) {
+          uint32_t raw[32];
+          tmem_ld_32x32(acc_row() + c * 32, raw);
+          do_chunk(c, raw);
         }
       }
-      if (!SPLIT && ++acc == NS_ACC) { acc = 0; acc_ph ^= 1; }
+      if (!ok) break;
+      // this warp's part of the tile is written: count it
+      if (elect_one()) {
+        bulk_wait_all();
+        fence_proxy_async_global();
+        __threadfence();
+        asm volatile("red.release.gpu.global.add.u32 [%0], 1;" ::"l"(g.done + t.z) : "memory");
+      }
+      __syncwarp();
     }
-    if (elect_one()) bulk_wait_all();      // the stores are complete before the kernel ends
+    if (elect_one()) bulk_wait_all();
     __syncwarp();
   }
 
@@ -453,49 +609,29 @@ __device__ __forceinline__ void ns_product_body(const NsMaps& maps, const NsProd
   if (PAIR) cluster_sync_all();
   if (warp == 1) {
     tc_fence_after_sync();
-    if (PAIR) tmem_dealloc_pair(tmem_base, NS_ACC * ACC_COLS);
-    else tmem_dealloc(tmem_base, NS_ACC * ACC_COLS);
+    if (PAIR) tmem_dealloc_pair(tmem_base, NS_ACC * TILE);
+    else tmem_dealloc(tmem_base, NS_ACC * TILE);
   }
 }
 
 __global__ void __launch_bounds__(NS_THREADS, 1)
-ns_product_kernel(const __grid_constant__ NsMaps maps, const __grid_constant__ NsProduct g, Status* status) {
-  ns_product_body<false, false>(maps, g, status);
+ns_chain_kernel(const __grid_constant__ NsPlan g, Status* status) {
+  ns_chain_body<false, false>(g, status);
 }
 
 __global__ void __launch_bounds__(NS_THREADS, 1)
-ns_product_split_kernel(const __grid_constant__ NsMaps maps, const __grid_constant__ NsProduct g, Status* status) {
-  ns_product_body<false, true>(maps, g, status);
+ns_chain_split_kernel(const __grid_constant__ NsPlan g, Status* status) {
+  ns_chain_body<false, true>(g, status);
 }
 
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(NS_THREADS, 1)
-ns_product_pair_kernel(const __grid_constant__ NsMaps maps, const __grid_constant__ NsProduct g, Status* status) {
-  ns_product_body<true, false>(maps, g, status);
+ns_chain_pair_kernel(const __grid_constant__ NsPlan g, Status* status) {
+  ns_chain_body<true, false>(g, status);
 }
 
 // ---------------------------------------------------------------------------------------
 // element-wise ends: momentum, norm, scaling into the operand format, result
 // ---------------------------------------------------------------------------------------
-template <typename T>
-__device__ __forceinline__ float ns_f32(T v);
-template <>
-__device__ __forceinline__ float ns_f32<float>(float v) { return v; }
-template <>
-__device__ __forceinline__ float ns_f32<__half>(__half v) { return __half2float(v); }
-template <>
-__device__ __forceinline__ float ns_f32<__nv_bfloat16>(__nv_bfloat16 v) { return __bfloat162float(v); }
-
-__device__ __forceinline__ float load_elem(const void* p, int dtype, int64_t i) {
-  if (dtype == ELEM_F32) return reinterpret_cast<const float*>(p)[i];
-  if (dtype == ELEM_BF16) return ns_f32(reinterpret_cast<const __nv_bfloat16*>(p)[i]);
-  return ns_f32(reinterpret_cast<const __half*>(p)[i]);
-}
-__device__ __forceinline__ void store_elem(void* p, int dtype, int64_t i, float v) {
-  if (dtype == ELEM_F32) reinterpret_cast<float*>(p)[i] = v;
-  else if (dtype == ELEM_BF16) reinterpret_cast<__nv_bfloat16*>(p)[i] = __float2bfloat16_rn(v);
-  else reinterpret_cast<__half*>(p)[i] = __float2half_rn(v);
-}
-
 __device__ __forceinline__ double block_sum(double v, double* red) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
@@ -507,71 +643,197 @@ __device__ __forceinline__ double block_sum(double v, double* red) {
   return s;
 }
 
+// Rows are covered by 2^tpr_log2 threads in steps of V elements, so no index is divided; a block takes ENDS_ROWS rows per
+// thread group at a time, whose loads are in flight together.
+constexpr int ENDS_THREADS = 256;
+constexpr int ENDS_ROWS = 4;
+
+template <int V>
+struct alignas(V * 4) VecF { float e[V]; };
+template <int V>
+struct alignas(V * 2) VecH { uint16_t e[V]; };
+
+template <int V>
+__device__ __forceinline__ VecF<V> load_vec(const void* p, int dtype, int64_t i) {
+  VecF<V> v;
+  if (dtype == ELEM_F32) return *reinterpret_cast<const VecF<V>*>(reinterpret_cast<const float*>(p) + i);
+  const VecH<V> h = *reinterpret_cast<const VecH<V>*>(reinterpret_cast<const uint16_t*>(p) + i);
+#pragma unroll
+  for (int q = 0; q < V; ++q)
+    v.e[q] = dtype == ELEM_BF16 ? __uint_as_float((uint32_t)h.e[q] << 16) : __half2float(__ushort_as_half(h.e[q]));
+  return v;
+}
+template <int V>
+__device__ __forceinline__ void store_vec(void* p, int dtype, int64_t i, const VecF<V>& v) {
+  if (dtype == ELEM_F32) {
+    *reinterpret_cast<VecF<V>*>(reinterpret_cast<float*>(p) + i) = v;
+    return;
+  }
+  VecH<V> h;
+#pragma unroll
+  for (int q = 0; q < V; ++q)
+    h.e[q] = dtype == ELEM_BF16 ? __bfloat16_as_ushort(__float2bfloat16_rn(v.e[q])) : __half_as_ushort(__float2half_rn(v.e[q]));
+  *reinterpret_cast<VecH<V>*>(reinterpret_cast<uint16_t*>(p) + i) = h;
+}
+
+// Sum of squares without overflow or underflow: fp32 where the largest of the values allows it, fp64 otherwise.
+template <int V>
+__device__ __forceinline__ void add_squares(double& ssq, const VecF<V>& u) {
+  float top = 0.0f, s = 0.0f;
+#pragma unroll
+  for (int q = 0; q < V; ++q) {
+    top = fmaxf(top, fabsf(u.e[q]));
+    s = fmaf(u.e[q], u.e[q], s);
+  }
+  if (top > 1e-16f && top < 1e18f) {
+    ssq += (double)s;
+  } else {
+#pragma unroll
+    for (int q = 0; q < V; ++q) ssq += (double)u.e[q] * (double)u.e[q];
+  }
+}
+
 // u (fp32, row pitch ld) of every matrix and the blocks' partial sums of u^2. Without momentum u is the input itself.
 //   g = scalars[1] * ((1 - beta * scalars[0]) * gt + beta * gi);   m <- mu m + g;   u = nesterov ? g + mu m : m
-__global__ void __launch_bounds__(256)
+template <int V>
+__global__ void __launch_bounds__(ENDS_THREADS)
 ns_begin_kernel(const __grid_constant__ NsEnds e) {
-  __shared__ double red[8];
+  __shared__ double red[ENDS_THREADS / 32];
   const int z = blockIdx.y;
-  const int64_t numel = (int64_t)e.rows * e.cols;
+  const int group = threadIdx.x >> e.tpr_log2, groups = ENDS_THREADS >> e.tpr_log2;
+  const int c0 = (threadIdx.x & ((1 << e.tpr_log2) - 1)) * V;
+  if (blockIdx.x == 0 && threadIdx.x == 0) {
+    e.done[z] = 0;
+    if (z == 0) *e.next_item = 0;
+  }
   float kt = 1.0f, ki = 0.0f;
   if (e.scalars != nullptr) {
     kt = (1.0f - e.beta * e.scalars[0]) * e.scalars[1];
     ki = e.beta * e.scalars[1];
   }
+  const void* gt = e.grad[z];
+  const void* gi = e.info[z];
+  float* mom = reinterpret_cast<float*>(e.moment[z]);
+  float* up = e.u + (int64_t)z * e.plane;
   double ssq = 0.0;
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < numel; i += (int64_t)gridDim.x * 256) {
-    const int64_t r = i / e.cols, c = i - r * e.cols;
-    float u;
-    if (e.momentum) {
-      float g = load_elem(e.grad[z], e.grad_dtype, i);
-      if (e.scalars != nullptr) {
-        g *= kt;
-        if (e.info[z] != nullptr) g = fmaf(ki, load_elem(e.info[z], e.grad_dtype, i), g);
+  for (int r0 = blockIdx.x * groups * ENDS_ROWS; r0 < e.rows; r0 += gridDim.x * groups * ENDS_ROWS) {
+    for (int c = c0; c < e.cols; c += V << e.tpr_log2) {
+      VecF<V> g[ENDS_ROWS], f[ENDS_ROWS], m[ENDS_ROWS];
+#pragma unroll
+      for (int q = 0; q < ENDS_ROWS; ++q) {
+        const int r = r0 + q * groups + group;
+        if (r >= e.rows) continue;
+        g[q] = load_vec<V>(gt, e.grad_dtype, (int64_t)r * e.grad_ld + c);
+        if (e.momentum) {
+          m[q] = *reinterpret_cast<const VecF<V>*>(mom + (int64_t)r * e.cols + c);
+          if (gi != nullptr) f[q] = load_vec<V>(gi, e.grad_dtype, (int64_t)r * e.grad_ld + c);
+        }
       }
-      float* mp = reinterpret_cast<float*>(e.moment[z]);
-      const float m = fmaf(e.mu, mp[i], g);
-      mp[i] = m;
-      u = e.nesterov ? fmaf(e.mu, m, g) : m;
-    } else {
-      u = load_elem(e.grad[z], e.grad_dtype, r * e.grad_ld + c);
+#pragma unroll
+      for (int q = 0; q < ENDS_ROWS; ++q) {
+        const int r = r0 + q * groups + group;
+        if (r >= e.rows) continue;
+        VecF<V> u = g[q];
+        if (e.momentum) {
+#pragma unroll
+          for (int i = 0; i < V; ++i) {
+            float x = g[q].e[i];
+            if (e.scalars != nullptr) {
+              x *= kt;
+              if (gi != nullptr) x = fmaf(ki, f[q].e[i], x);
+            }
+            m[q].e[i] = fmaf(e.mu, m[q].e[i], x);
+            u.e[i] = e.nesterov ? fmaf(e.mu, m[q].e[i], x) : m[q].e[i];
+          }
+          *reinterpret_cast<VecF<V>*>(mom + (int64_t)r * e.cols + c) = m[q];
+        }
+        *reinterpret_cast<VecF<V>*>(up + (int64_t)r * e.ld + c) = u;
+        add_squares<V>(ssq, u);
+      }
     }
-    e.u[(int64_t)z * e.plane + r * e.ld + c] = u;
-    ssq += (double)u * (double)u;
   }
   const double s = block_sum(ssq, red);
   if (threadIdx.x == 0) e.partial[(int64_t)z * gridDim.x + blockIdx.x] = s;
 }
 
 // u / (norm + eps) * 2^14 as hi + lo
-__global__ void __launch_bounds__(256)
+template <int V>
+__global__ void __launch_bounds__(ENDS_THREADS)
 ns_scale_kernel(const __grid_constant__ NsEnds e, int n_partial) {
   const int z = blockIdx.y;
+  const int group = threadIdx.x >> e.tpr_log2, groups = ENDS_THREADS >> e.tpr_log2;
+  const int c0 = (threadIdx.x & ((1 << e.tpr_log2) - 1)) * V;
   double s = 0.0;
-  for (int i = 0; i < n_partial; ++i) s += e.partial[(int64_t)z * n_partial + i];
+  for (int i = threadIdx.x & 31; i < n_partial; i += 32) s += e.partial[(int64_t)z * n_partial + i];
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
   const double inv = (double)NS_SCALE / (sqrt(s) + (double)e.eps);
-  const int64_t numel = (int64_t)e.rows * e.ld;
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < numel; i += (int64_t)gridDim.x * 256) {
-    if (i % e.ld >= e.cols) continue;
-    const int64_t at = (int64_t)z * e.plane + i;
-    const float v = (float)((double)e.u[at] * inv);
-    const __half h = __float2half_rn(v);
-    e.x_hi[at] = h;
-    e.x_lo[at] = __float2half_rn(v - __half2float(h));
+  const float finv = (float)inv;
+  const bool fine = finv > 1e-30f && finv < 1e30f;      // else the factor itself does not fit fp32
+  const float* up = e.u + (int64_t)z * e.plane;
+  __half* hi = e.x_hi + (int64_t)z * e.plane;
+  __half* lo = e.x_lo + (int64_t)z * e.plane;
+  for (int r0 = blockIdx.x * groups * ENDS_ROWS; r0 < e.rows; r0 += gridDim.x * groups * ENDS_ROWS) {
+    for (int c = c0; c < e.cols; c += V << e.tpr_log2) {
+      VecF<V> u[ENDS_ROWS];
+#pragma unroll
+      for (int q = 0; q < ENDS_ROWS; ++q) {
+        const int r = r0 + q * groups + group;
+        if (r < e.rows) u[q] = *reinterpret_cast<const VecF<V>*>(up + (int64_t)r * e.ld + c);
+      }
+#pragma unroll
+      for (int q = 0; q < ENDS_ROWS; ++q) {
+        const int r = r0 + q * groups + group;
+        if (r >= e.rows) continue;
+        VecH<V> h, l;
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+          const float v = fine ? u[q].e[i] * finv : (float)((double)u[q].e[i] * inv);
+          const __half a = __float2half_rn(v);
+          h.e[i] = __half_as_ushort(a);
+          l.e[i] = __half_as_ushort(__float2half_rn(v - __half2float(a)));
+        }
+        *reinterpret_cast<VecH<V>*>(hi + (int64_t)r * e.ld + c) = h;
+        *reinterpret_cast<VecH<V>*>(lo + (int64_t)r * e.ld + c) = l;
+      }
+    }
   }
 }
 
 // the result, or the parameter update p <- p * decay - step * x
-__global__ void __launch_bounds__(256)
+template <int V>
+__global__ void __launch_bounds__(ENDS_THREADS)
 ns_end_kernel(const __grid_constant__ NsEnds e) {
   const int z = blockIdx.y;
-  const int64_t numel = (int64_t)e.rows * e.cols;
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < numel; i += (int64_t)gridDim.x * 256) {
-    const int64_t r = i / e.cols, c = i - r * e.cols;
-    const int64_t at = (int64_t)z * e.plane + r * e.ld + c;
-    const float x = (__half2float(e.x_hi[at]) + __half2float(e.x_lo[at])) * NS_UNSCALE;
-    if (e.momentum) store_elem(e.out[z], e.out_dtype, i, fmaf(-e.step, x, load_elem(e.out[z], e.out_dtype, i) * e.decay));
-    else store_elem(e.out[z], e.out_dtype, i, x);
+  const int group = threadIdx.x >> e.tpr_log2, groups = ENDS_THREADS >> e.tpr_log2;
+  const int c0 = (threadIdx.x & ((1 << e.tpr_log2) - 1)) * V;
+  const __half* hi = e.x_hi + (int64_t)z * e.plane;
+  const __half* lo = e.x_lo + (int64_t)z * e.plane;
+  void* out = e.out[z];
+  for (int r0 = blockIdx.x * groups * ENDS_ROWS; r0 < e.rows; r0 += gridDim.x * groups * ENDS_ROWS) {
+    for (int c = c0; c < e.cols; c += V << e.tpr_log2) {
+      VecF<V> p[ENDS_ROWS];
+      VecH<V> h[ENDS_ROWS], l[ENDS_ROWS];
+#pragma unroll
+      for (int q = 0; q < ENDS_ROWS; ++q) {
+        const int r = r0 + q * groups + group;
+        if (r >= e.rows) continue;
+        h[q] = *reinterpret_cast<const VecH<V>*>(hi + (int64_t)r * e.ld + c);
+        l[q] = *reinterpret_cast<const VecH<V>*>(lo + (int64_t)r * e.ld + c);
+        if (e.momentum) p[q] = load_vec<V>(out, e.out_dtype, (int64_t)r * e.cols + c);
+      }
+#pragma unroll
+      for (int q = 0; q < ENDS_ROWS; ++q) {
+        const int r = r0 + q * groups + group;
+        if (r >= e.rows) continue;
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+          const float x = (__half2float(__ushort_as_half(h[q].e[i])) + __half2float(__ushort_as_half(l[q].e[i]))) * NS_UNSCALE;
+          p[q].e[i] = e.momentum ? fmaf(-e.step, x, p[q].e[i] * e.decay) : x;
+        }
+        store_vec<V>(out, e.out_dtype, (int64_t)r * e.cols + c, p[q]);
+      }
+    }
   }
 }
 
@@ -610,7 +872,7 @@ static bool ns_map(CUtensorMap* out, const __half* base, int64_t batch, int64_t 
 
 static int64_t ns_ld(int64_t cols) { return (cols + 31) / 32 * 32; }   // the epilogue reads whole 32-column chunks
 
-// Layout of the workspace for `batch` matrices: X twice (hi and lo planes), A and B (hi and lo), norms.
+// Layout of the workspace for `batch` matrices: X twice (hi and lo planes), A and B (hi and lo), norms, tile counts.
 struct NsSpace {
   int64_t ld_x, plane_x, ld_k, plane_k, x, k, partial, total;   // elements; x, k = one buffer's hi + lo
 };
@@ -624,24 +886,16 @@ static NsSpace ns_space(int64_t batch, int64_t rows, int64_t cols) {
   w.x = 2 * batch * w.plane_x;
   w.k = 2 * batch * w.plane_k;
   w.partial = 2 * w.x + 2 * w.k;                                // byte offset = 2 * elements, a multiple of 64
-  w.total = 2 * w.partial + batch * NS_NORM_BLOCKS * (int64_t)sizeof(double);
+  w.total = 2 * w.partial + batch * NS_NORM_BLOCKS * (int64_t)sizeof(double) + (batch + 1) * (int64_t)sizeof(uint32_t);
   return w;
 }
 
 int64_t ns_workspace_bytes(int64_t batch, int64_t rows, int64_t cols) { return ns_space(batch, rows, cols).total; }
 
-static const char* ns_launch_product(const NsMaps& maps, const NsProduct& g, bool pair, int sms, Status* status, cudaStream_t st) {
-  const int work = g.batch * g.tiles;
-  if (pair) {
-    const int units = sms / 2 < work ? sms / 2 : work;
-    if (launch_pdl(ns_product_pair_kernel, dim3(2 * units), dim3(NS_THREADS), NS_SMEM, st, maps, g, status) != cudaSuccess)
-      return "ns_product_pair launch failed";
-  } else {
-    const int units = sms < work ? sms : work;
-    if (launch_pdl(g.pairs ? ns_product_split_kernel : ns_product_kernel, dim3(units), dim3(NS_THREADS), NS_SMEM, st, maps, g, status) != cudaSuccess)
-      return "ns_product launch failed";
-  }
-  return nullptr;
+template <int V>
+static void ns_begin(const NsEnds& e, int norm_blocks, int blocks, cudaStream_t st) {
+  ns_begin_kernel<V><<<dim3(norm_blocks, e.batch), ENDS_THREADS, 0, st>>>(e);
+  ns_scale_kernel<V><<<dim3(blocks, e.batch), ENDS_THREADS, 0, st>>>(e, norm_blocks);
 }
 
 const char* launch_orthogonalize(const NsCall& call, Status* status, cudaStream_t st) {
@@ -654,121 +908,104 @@ const char* launch_orthogonalize(const NsCall& call, Status* status, cudaStream_
   __half* A = base + 2 * w.x;
   __half* B = A + w.k;
   const int64_t lo_x = w.x / 2, lo_k = w.k / 2;
+  uint8_t* tail = reinterpret_cast<uint8_t*>(call.workspace) + 2 * w.partial;
   const bool tall = rows > cols;
-  const int k = (int)(tall ? cols : rows);
 
-  int dev = 0, sms = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
+  int dev = 0, sms = 0, l2 = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess ||
+      cudaDeviceGetAttribute(&l2, cudaDevAttrL2CacheSize, dev) != cudaSuccess)
     return "orthogonalize: device";
 
+  NsPlan g;
+  memset(&g, 0, sizeof(g));
   NsEnds e = call.ends;
   e.ld = (int)w.ld_x;
   e.plane = w.plane_x;
   e.u = reinterpret_cast<float*>(x[1]);                    // hi and lo planes of the other X buffer: four bytes an element
   e.x_hi = x[0];
   e.x_lo = x[0] + lo_x;
-  e.partial = reinterpret_cast<double*>(reinterpret_cast<uint8_t*>(call.workspace) + 2 * w.partial);
-  const int64_t numel = rows * cols;
-  int64_t blocks = (numel + 2047) / 2048;
+  e.partial = reinterpret_cast<double*>(tail);
+  e.done = reinterpret_cast<uint32_t*>(tail + batch * NS_NORM_BLOCKS * sizeof(double));
+  e.next_item = e.done + batch;
+  // four elements an access where every row of every matrix allows it
+  const int in_size = e.grad_dtype == ELEM_F32 ? 4 : 2, out_size = e.out_dtype == ELEM_F32 ? 4 : 2;
+  bool vec = cols % 4 == 0 && e.grad_ld % 4 == 0;
+  for (int64_t z = 0; z < batch && vec; ++z) {
+    vec = reinterpret_cast<uintptr_t>(e.grad[z]) % (4 * in_size) == 0 && reinterpret_cast<uintptr_t>(e.out[z]) % (4 * out_size) == 0 &&
+          reinterpret_cast<uintptr_t>(e.info[z]) % (4 * in_size) == 0 && reinterpret_cast<uintptr_t>(e.moment[z]) % 16 == 0;
+  }
+  const int64_t per_row = (cols + (vec ? 3 : 0)) / (vec ? 4 : 1);
+  e.tpr_log2 = 0;
+  while (e.tpr_log2 < 8 && (1 << e.tpr_log2) < per_row) ++e.tpr_log2;
+  const int64_t rows_per_block = (ENDS_THREADS >> e.tpr_log2) * ENDS_ROWS;
+  const int64_t blocks = (rows + rows_per_block - 1) / rows_per_block;
   const int norm_blocks = (int)(blocks < NS_NORM_BLOCKS ? blocks : NS_NORM_BLOCKS);
-  blocks = blocks < 1024 ? blocks : 1024;
-  ns_begin_kernel<<<dim3(norm_blocks, (unsigned)batch), 256, 0, st>>>(e);
-  ns_scale_kernel<<<dim3((unsigned)blocks, (unsigned)batch), 256, 0, st>>>(e, norm_blocks);
+  const int all_blocks = (int)(blocks < 4096 ? blocks : 4096);
+  if (vec) ns_begin<4>(e, norm_blocks, all_blocks, st);
+  else ns_begin<1>(e, norm_blocks, all_blocks, st);
 
-  if (cudaFuncSetAttribute(ns_product_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, NS_SMEM) != cudaSuccess ||
-      cudaFuncSetAttribute(ns_product_split_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, NS_SMEM) != cudaSuccess ||
-      cudaFuncSetAttribute(ns_product_pair_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, NS_SMEM) != cudaSuccess)
-    return "orthogonalize: shared memory";
-
+  g.batch = (int)batch;
+  g.steps = call.steps;
+  g.rows = (int)rows;
+  g.cols = (int)cols;
+  g.tall = tall;
+  g.k = (int)(tall ? cols : rows);
+  g.wide = (int)(tall ? rows : cols);
+  g.a = call.c[0];
+  g.b = call.c[1];
+  g.c = call.c[2];
+  g.done = e.done;
+  g.next_item = e.next_item;
   // A pair's 256 x 256 tile needs half the operand traffic of a 128 x 128 one; with a side of 256 or less it would leave one
   // or two pairs to work on each matrix.
-  const bool pair = k > 256 && !call.pairs;
+  const bool pair = g.k > 256 && !call.pairs;
   const int tile = pair ? 256 : 128;
-  auto load_map = [&](CUtensorMap* m, const __half* p, int64_t r, int64_t c, int64_t ld, int64_t plane, bool mn) {
-    return ns_map(m, p, batch, r, c, ld, plane, mn ? NS_BK : 128, 64, CU_TENSOR_MAP_SWIZZLE_128B);
-  };
-  auto store_map = [&](CUtensorMap* m, const __half* p, int64_t r, int64_t c, int64_t ld, int64_t plane) {
-    return ns_map(m, p, batch, r, c, ld, plane, NS_BOX, NS_BOX, CU_TENSOR_MAP_SWIZZLE_64B);
-  };
-  const int kt = (k + tile - 1) / tile, wt = (int)(((tall ? rows : cols) + tile - 1) / tile);
-  int cur = 0;
-  for (int step = 0; step < call.steps; ++step) {
-    __half* xin = x[cur];
-    __half* xout = x[cur ^ 1];
-    NsMaps m1, m2, m3;
-    bool ok = true;
-    // A = X X^T (wide: X rows are K-major; tall: A = X^T X, both operands MN-major)
-    ok &= load_map(&m1.p_hi, xin, rows, cols, w.ld_x, w.plane_x, tall);
-    ok &= load_map(&m1.p_lo, xin + lo_x, rows, cols, w.ld_x, w.plane_x, tall);
-    m1.q_hi = m1.p_hi;
-    m1.q_lo = m1.p_lo;
-    ok &= store_map(&m1.out_hi, A, k, k, w.ld_k, w.plane_k);
-    ok &= store_map(&m1.out_lo, A + lo_k, k, k, w.ld_k, w.plane_k);
-    // B = b A + c A A^T
-    ok &= load_map(&m2.p_hi, A, k, k, w.ld_k, w.plane_k, false);
-    ok &= load_map(&m2.p_lo, A + lo_k, k, k, w.ld_k, w.plane_k, false);
-    m2.q_hi = m2.p_hi;
-    m2.q_lo = m2.p_lo;
-    ok &= store_map(&m2.out_hi, B, k, k, w.ld_k, w.plane_k);
-    ok &= store_map(&m2.out_lo, B + lo_k, k, k, w.ld_k, w.plane_k);
-    // X' = a X + B X (wide: X is the MN-major second operand) or a X + X B^T (tall)
-    CUtensorMap b_hi, b_lo;
-    ok &= load_map(&b_hi, B, k, k, w.ld_k, w.plane_k, false);
-    ok &= load_map(&b_lo, B + lo_k, k, k, w.ld_k, w.plane_k, false);
-    CUtensorMap x_hi, x_lo;
-    ok &= load_map(&x_hi, xin, rows, cols, w.ld_x, w.plane_x, !tall);
-    ok &= load_map(&x_lo, xin + lo_x, rows, cols, w.ld_x, w.plane_x, !tall);
-    m3.p_hi = tall ? x_hi : b_hi;
-    m3.p_lo = tall ? x_lo : b_lo;
-    m3.q_hi = tall ? b_hi : x_hi;
-    m3.q_lo = tall ? b_lo : x_lo;
-    ok &= store_map(&m3.out_hi, xout, rows, cols, w.ld_x, w.plane_x);
-    ok &= store_map(&m3.out_lo, xout + lo_x, rows, cols, w.ld_x, w.plane_x);
-    if (!ok) return "orthogonalize: cuTensorMapEncodeTiled failed";
+  const int kt = (g.k + tile - 1) / tile, wt = (g.wide + tile - 1) / tile;
+  g.tiles_sym = kt * (kt + 1) / 2;
+  g.tiles_x = kt * wt;
+  g.tiles_xm = tall ? wt : kt;
+  const int units = pair ? sms / 2 : sms;
+  // as many matrices as L2 holds with their two X buffers, A and B, but enough tiles to keep every unit busy twice
+  const int64_t bytes = 2 * (w.x * 2 + w.k * (call.pairs ? 2 : 1)) / batch;
+  int64_t window = l2 / bytes;
+  const int64_t least = (2 * units + g.tiles_sym - 1) / g.tiles_sym;
+  if (window < least) window = least;
+  g.window = (int)(window < batch ? window : batch);
+  const int64_t items = batch * g.steps * (2 * g.tiles_sym + g.tiles_x);
+  if (items > (1ll << 30)) return "orthogonalize: too many tiles";
+  g.items = (int)items;
 
-    NsProduct g{};
-    g.batch = (int)batch;
-    g.pairs = call.pairs;
-    g.M = g.N = k;
-    g.K = (int)(tall ? rows : cols);
-    g.symmetric = 1;
-    g.p_mn = g.q_mn = tall;
-    g.store_lo = call.pairs;
-    g.acc_scale = NS_UNSCALE;
-    g.tiles_m = kt;
-    g.tiles = kt * (kt + 1) / 2;
-    const char* err = ns_launch_product(m1, g, pair, sms, status, st);
-    if (err) return err;
-    g.K = k;
-    g.p_mn = g.q_mn = 0;
-    g.acc_scale = call.c[2] * NS_UNSCALE;
-    g.aux_scale = call.c[1];
-    g.aux_hi = A;
-    g.aux_lo = call.pairs ? A + lo_k : nullptr;
-    g.aux_ld = w.ld_k;
-    g.aux_stride = w.plane_k;
-    err = ns_launch_product(m2, g, pair, sms, status, st);
-    if (err) return err;
-    g.M = (int)rows;
-    g.N = (int)cols;
-    g.symmetric = 0;
-    g.q_mn = !tall;
-    g.store_lo = 1;
-    g.acc_scale = NS_UNSCALE;
-    g.aux_scale = call.c[0];
-    g.aux_hi = xin;
-    g.aux_lo = xin + lo_x;
-    g.aux_ld = w.ld_x;
-    g.aux_stride = w.plane_x;
-    g.tiles_m = tall ? wt : kt;
-    g.tiles = kt * wt;
-    err = ns_launch_product(m3, g, pair, sms, status, st);
-    if (err) return err;
-    cur ^= 1;
+  bool ok = true;
+  auto load_map = [&](CUtensorMap* m, const __half* p, int64_t r, int64_t c, int64_t ld, int64_t plane, bool mn) {
+    ok &= ns_map(m, p, batch, r, c, ld, plane, mn ? NS_BK : 128, 64, CU_TENSOR_MAP_SWIZZLE_128B);
+  };
+  auto box_map = [&](CUtensorMap* m, const __half* p, int64_t r, int64_t c, int64_t ld, int64_t plane) {
+    ok &= ns_map(m, p, batch, r, c, ld, plane, NS_BOX, NS_BOX, CU_TENSOR_MAP_SWIZZLE_64B);
+  };
+  for (int lo = 0; lo < 2; ++lo) {
+    for (int i = 0; i < 2; ++i) {
+      const __half* p = x[i] + lo * lo_x;
+      load_map(&g.x_gram[i][lo], p, rows, cols, w.ld_x, w.plane_x, tall);      // A = X X^T; tall: X^T X, both operands MN-major
+      load_map(&g.x_apply[i][lo], p, rows, cols, w.ld_x, w.plane_x, !tall);    // B X: X is the MN-major second operand; tall: X B^T
+      box_map(&g.x_box[i][lo], p, rows, cols, w.ld_x, w.plane_x);
+    }
+    load_map(&g.a_load[lo], A + lo * lo_k, g.k, g.k, w.ld_k, w.plane_k, false);
+    load_map(&g.b_load[lo], B + lo * lo_k, g.k, g.k, w.ld_k, w.plane_k, false);
+    box_map(&g.a_box[lo], A + lo * lo_k, g.k, g.k, w.ld_k, w.plane_k);
+    box_map(&g.b_box[lo], B + lo * lo_k, g.k, g.k, w.ld_k, w.plane_k);
   }
-  e.x_hi = x[cur];
-  e.x_lo = x[cur] + lo_x;
-  ns_end_kernel<<<dim3((unsigned)blocks, (unsigned)batch), 256, 0, st>>>(e);
+  if (!ok) return "orthogonalize: cuTensorMapEncodeTiled failed";
+  if (g.items > 0) {
+    auto kernel = call.pairs ? ns_chain_split_kernel : (pair ? ns_chain_pair_kernel : ns_chain_kernel);
+    const int smem = call.pairs ? NsShape<true>::SMEM : NsShape<false>::SMEM;
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) return "orthogonalize: shared memory";
+    const int most = (int)(batch * g.tiles_x < units ? batch * g.tiles_x : units);      // no product has more tiles at once than that
+    kernel<<<(pair ? 2 : 1) * most, NS_THREADS, smem, st>>>(g, status);
+  }
+  e.x_hi = x[g.steps & 1];
+  e.x_lo = x[g.steps & 1] + lo_x;
+  if (vec) ns_end_kernel<4><<<dim3(all_blocks, (unsigned)batch), ENDS_THREADS, 0, st>>>(e);
+  else ns_end_kernel<1><<<dim3(all_blocks, (unsigned)batch), ENDS_THREADS, 0, st>>>(e);
   return cudaGetLastError() == cudaSuccess ? nullptr : "orthogonalize launch failed";
 }
 

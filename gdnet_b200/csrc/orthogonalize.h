@@ -31,21 +31,22 @@ struct NsEnds {
   double* partial;
   __half* x_hi;
   __half* x_lo;
+  int tpr_log2;                        // threads per row (log2)
+  uint32_t* done;                      // tile counts, cleared by the first kernel of a call
+  uint32_t* next_item;
 };
 
-struct NsMaps {
-  CUtensorMap p_hi, p_lo, q_hi, q_lo, out_hi, out_lo;
-};
-
-// One product over the batch (see ns_product_body)
-struct NsProduct {
-  int batch, M, N, K;
-  int symmetric, pairs, p_mn, q_mn, store_lo;
-  int tiles, tiles_m;                  // tiles of one matrix; row blocks
-  float acc_scale, aux_scale;
-  const __half* aux_hi;
-  const __half* aux_lo;
-  int64_t aux_ld, aux_stride;
+// All products of a call (see ns_chain_body). Tensor maps [buffer][hi, lo].
+struct NsPlan {
+  CUtensorMap x_gram[2][2], x_apply[2][2], x_box[2][2];
+  CUtensorMap a_load[2], a_box[2], b_load[2], b_box[2];
+  int batch, steps, rows, cols, tall;
+  int k, wide;                         // smaller and larger side
+  int tiles_sym, tiles_x, tiles_xm;    // tiles of a symmetric product, of X, row blocks of X
+  int window, items;
+  float a, b, c;
+  uint32_t* done;                      // [batch] finished tiles, counted in epilogue warps
+  uint32_t* next_item;
 };
 
 struct NsCall {
