@@ -5,8 +5,8 @@
 //     A = X X^T,   B = b A + c A^2,   X <- a X + B X          (r <= c; otherwise A = X^T X and X <- a X + X B)
 //
 // which moves every singular value s to s (a + b s^2 + c s^4) and keeps the singular vectors. Three products a step, the
-// first two symmetric: only the tiles on and above the diagonal are computed and their transposes stored from the same
-// registers, so a step costs k (k + 1) w + k (k + 1) k + 2 k^2 w operations with k = min(r, c), w = max(r, c), against
+// first two symmetric: only the tiles on and above the diagonal of A and B are computed and stored, and what lies below is
+// read from above with the operand's other major order (a bit of the MMA instruction), so a step costs k (k + 1) w + k (k + 1) k + 2 k^2 w operations with k = min(r, c), w = max(r, c), against
 // 4 k^2 w + 2 k^3 without. Bound by the tensor cores from about k = 1024 on, by the latency of 3 x steps dependent
 // products below.
 //
@@ -59,42 +59,46 @@ __device__ __forceinline__ void tma_store_3d(const CUtensorMap* m, uint32_t src,
 // item waits only for items before it: the products of a matrix follow one another, and a count of the finished
 // tiles per matrix says how far it is. So any number of resident blocks makes progress (two calls on two streams may share
 // the GPU), nothing is launched between the 3 x steps products, and the tiles of one product fill the gaps that
-// the end of another leaves. The order is: for a window of matrices, product by product, all their tiles; a window is as many
-// matrices as stay in L2 from one product to the next.
+// the end of another leaves. The order is: product by product, all matrices. (Windows of as many matrices as stay in L2 from
+// one product to the next were slower: 48 matrices of 1024 x 1024 take 1.69 ms as one window, 2.07 in windows of 8, whose ends
+// wait on one another.)
 //
-// A block: warp 0 fetches items and loads operands with bulk tensor copies into a ring of stages; warp 1 issues the MMAs into
-// two accumulators in TMEM; eight epilogue warps read the accumulator, add the linear term (its boxes are copied in
-// while the MMAs run) and send 32 x 32 boxes out with bulk stores. PAIR: a pair of CTAs on two SMs shares a
+// A block: warp 10 fetches items, waits until what they read is written and hands them to the others; warp 0 loads operands
+// with bulk tensor copies into a ring of stages; warp 1 issues the MMAs into two accumulators in TMEM; warps 2..9
+// read the accumulator, add the linear term (its boxes are copied in while the MMAs run) and send 32 x 32 boxes
+// out with bulk stores. A diagonal tile of a symmetric product reads the same rows twice and loads them once. PAIR: a pair of CTAs on two SMs shares a
 // 256 x 256 tile, each loading its half of both operands; otherwise a CTA has a 128 x 128 tile of its own.
 constexpr int NS_BK = 64;                       // K elements per stage: one 128-byte swizzle row
 constexpr int NS_EPI_WARPS = 8;
-constexpr int NS_THREADS = 64 + NS_EPI_WARPS * 32;
+constexpr int NS_THREADS = 96 + NS_EPI_WARPS * 32;
 constexpr int NS_OPERAND_BYTES = 128 * 128;     // 128 rows x 64 fp16 per CTA and operand
 constexpr int NS_STAGE_BYTES = 2 * NS_OPERAND_BYTES;
 constexpr int NS_BOX = 32;                      // epilogue chunk: 32 x 32
 constexpr int NS_BOX_BYTES = NS_BOX * NS_BOX * 2;
-constexpr int NS_SLOTS = 2;                     // chunks in flight per epilogue warp
+constexpr int NS_SLOTS = 2;                     // chunks of the linear term in flight per epilogue warp
 constexpr int NS_ACC = 2;
 constexpr int NS_SPLIT_KBLOCKS = 2;             // pairs: K blocks summed in TMEM before the sum moves to registers
-// Items on their way through a block: the loads run at most the stages (5) ahead of the MMAs, these two accumulators ahead
-// of the epilogue, and one item is fetched early; a ring of 16 is never overwritten before it is read.
+// Items on their way through a block: two are handed out ahead of the loads, which run at most the stages (4) ahead of the
+// MMAs, these two accumulators ahead of the epilogue; a ring of 16 is never overwritten before it is read.
 constexpr int NS_RING = 16;
 
 template <bool SPLIT>
 struct NsShape {
-  static constexpr int STAGES = SPLIT ? 3 : 5;
-  static constexpr int SLOT_BOXES = SPLIT ? 4 : 2;               // (hi, transpose | lo), with pairs (hi, lo and both transposes)
-  static constexpr int WARP_BYTES = NS_SLOTS * SLOT_BOXES * NS_BOX_BYTES;
+  static constexpr int STAGES = 4;
+  static constexpr int AUX_BYTES = 2 * NS_BOX_BYTES;                          // hi and lo
+  static constexpr int OUT_BYTES = 2 * NS_BOX_BYTES;
+  static constexpr int WARP_BYTES = NS_SLOTS * AUX_BYTES + OUT_BYTES;
   static constexpr int SMEM = STAGES * NS_STAGE_BYTES + NS_EPI_WARPS * WARP_BYTES + 1024 + 1024;   // barriers; alignment
 };
 
 struct __align__(8) NsBars {
-  uint64_t full[5];
-  uint64_t empty[5];
+  uint64_t full[4];
+  uint64_t empty[4];
   uint64_t acc_full[NS_ACC];
   uint64_t acc_empty[NS_ACC];
   uint64_t aux_full[NS_EPI_WARPS * NS_SLOTS];
   uint64_t item_full[NS_RING];
+  uint64_t taken[2];                 // the loads have begun item it (barrier it & 1)
   int item[NS_RING];
   uint32_t tmem_base;
   int abort;
@@ -155,6 +159,14 @@ __device__ __forceinline__ int ns_next_item(NsBars* bars, int slot_no, Status* s
   return __shfl_sync(0xffffffffu, item, 0);
 }
 
+// Whether ns_next_item(slot_no) would return at once. Warp-collective.
+__device__ __forceinline__ bool ns_item_there(NsBars* bars, int slot_no) {
+  uint32_t ok = 0;
+  if ((threadIdx.x & 31) == 0)
+    ok = ns_try_wait_cluster(smem_u32(&bars->item_full[slot_no & (NS_RING - 1)]), (slot_no / NS_RING) & 1);
+  return __shfl_sync(0xffffffffu, ok, 0) != 0;
+}
+
 struct NsItem {
   int step, phase, z, mb, nb;        // phase 0: A, 1: B, 2: X
   uint32_t need;                     // finished tiles of matrix z that this one reads (in epilogue warps)
@@ -163,20 +175,15 @@ struct NsItem {
 __device__ __forceinline__ NsItem ns_decode(const NsPlan& g, int item, uint32_t warps_per_tile) {
   NsItem t;
   const int per_step = 2 * g.tiles_sym + g.tiles_x;
-  const int per_window = g.window * g.steps * per_step;
-  const int win = item / per_window;
-  int r = item - win * per_window;
-  const int z0 = win * g.window, count = min(g.window, g.batch - z0);
-  t.step = r / (count * per_step);
-  r -= t.step * count * per_step;
-  const int sym = count * g.tiles_sym;
+  t.step = item / (g.batch * per_step);
+  int r = item - t.step * g.batch * per_step;
+  const int sym = g.batch * g.tiles_sym;
   int tiles = g.tiles_sym;
   t.phase = 0;
   if (r >= 2 * sym) { t.phase = 2; r -= 2 * sym; tiles = g.tiles_x; }
   else if (r >= sym) { t.phase = 1; r -= sym; }
   t.z = r / tiles;
   r -= t.z * tiles;
-  t.z += z0;
   t.need = (uint32_t)(t.step * per_step + t.phase * g.tiles_sym) * warps_per_tile;
   if (t.phase == 2) {
     t.nb = r / g.tiles_xm;           // neighbours share a column block
@@ -215,22 +222,17 @@ __device__ __forceinline__ void ns_read_row(const uint8_t* box, int lane, uint32
     w[4 * q] = u.x; w[4 * q + 1] = u.y; w[4 * q + 2] = u.z; w[4 * q + 3] = u.w;
   }
 }
-// The transpose of the box: column j becomes row j. Neighbouring lanes exchange halves so that a store moves two rows' values.
-__device__ __forceinline__ void ns_write_transposed(uint8_t* box, int lane, const uint32_t (&w)[16]) {
-#pragma unroll
-  for (int t = 0; t < 16; ++t) {
-    const uint32_t other = __shfl_xor_sync(0xffffffffu, w[t], 1);
-    const uint32_t v = (lane & 1) ? __byte_perm(other, w[t], 0x7632) : __byte_perm(w[t], other, 0x5410);
-    *reinterpret_cast<uint32_t*>(box + ns_box_off(2 * t + (lane & 1), lane >> 3) + ((lane >> 1) & 3) * 4) = v;
-  }
-}
+// Whether K block kb (64 columns) of row block `block` of a symmetric factor lies below the diagonal, in tiles that are not
+// stored: it is then read as the transpose of the tile above.
+template <int TILE>
+__device__ __forceinline__ bool ns_below(int kb, int block) { return kb * NS_BK / TILE < block; }
 
 template <bool PAIR, bool SPLIT>
 __device__ __forceinline__ void ns_chain_body(const NsPlan& g, Status* status) {
   constexpr int TILE = PAIR ? 256 : 128;
   constexpr int CHUNKS = TILE / 64;              // 32-column chunks per epilogue warp (two warps share a lane quarter)
   constexpr int SEGS = SPLIT ? 3 : 1;
-  constexpr int STAGES = NsShape<SPLIT>::STAGES, SLOT_BOXES = NsShape<SPLIT>::SLOT_BOXES;
+  constexpr int STAGES = NsShape<SPLIT>::STAGES;
   constexpr uint32_t WARPS_PER_TILE = (PAIR ? 2 : 1) * NS_EPI_WARPS;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -250,6 +252,7 @@ __device__ __forceinline__ void ns_chain_body(const NsPlan& g, Status* status) {
     }
     for (int a = 0; a < NS_EPI_WARPS * NS_SLOTS; ++a) mbar_init(smem_u32(&bars->aux_full[a]), 1);
     for (int a = 0; a < NS_RING; ++a) mbar_init(smem_u32(&bars->item_full[a]), 1);
+    for (int a = 0; a < 2; ++a) mbar_init(smem_u32(&bars->taken[a]), 1);
     bars->abort = 0;
     fence_barrier_init();
   }
@@ -271,51 +274,27 @@ __device__ __forceinline__ void ns_chain_body(const NsPlan& g, Status* status) {
 
   if (warp == 0) {
     const uint32_t full_lead0 = PAIR ? map_to_cta(full0, 0) : full0;
-    const uint32_t peer_item0 = PAIR ? map_to_cta(smem_u32(&bars->item[0]), rank ^ 1) : 0;
-    const uint32_t peer_bar0 = PAIR ? map_to_cta(smem_u32(&bars->item_full[0]), rank ^ 1) : 0;
-    int s = 0, ahead = 0;
+    int s = 0;
     uint32_t ph = 0;
     bool ok = true;
-    if (rank == 0 && lane == 0) ahead = (int)atomicAdd(g.next_item, 1u);
     for (int it = 0; ok; ++it) {
-      int item;
-      if (rank == 0) {
-        item = __shfl_sync(0xffffffffu, ahead, 0);
-        if (item >= g.items || ns_aborted(bars)) item = -1;
-        if (lane == 0) {
-          const int slot = it & (NS_RING - 1);
-          *((volatile int*)&bars->item[slot]) = item;
-          mbar_arrive(smem_u32(&bars->item_full[slot]));
-          if (PAIR) {
-            ns_put_remote(peer_item0 + 4 * slot, item);
-            ns_arrive_remote(peer_bar0 + 8 * slot);
-          }
-          if (item >= 0) ahead = (int)atomicAdd(g.next_item, 1u);      // needed one item later
-        }
-        __syncwarp();
-      } else {
-        item = ns_next_item(bars, it, status);
-      }
+      const int item = ns_next_item(bars, it, status);
       if (item < 0) break;
+      if (rank == 0 && lane == 0) mbar_arrive(smem_u32(&bars->taken[it & 1]));
       const NsItem t = ns_decode(g, item, WARPS_PER_TILE);
-      uint32_t ready = 1;
-      if (lane == 0 && t.need != 0) ready = wait_flag_ge_gpu(g.done + t.z, t.need, GD_WAIT_BUDGET_NS);
-      if (!__shfl_sync(0xffffffffu, ready, 0)) {
-        if (lane == 0) ns_abort(bars, status, STATUS_TIMEOUT_PEER_FLAG, 84, t.z);
-        break;
-      }
       fence_proxy_async_global();      // what other blocks wrote before they counted up is read by bulk copies below
       const int cur = t.step & 1;
       const int m0 = t.mb * TILE + (int)rank * 128, n0 = t.nb * TILE + (int)rank * 128;
-      const bool p_mn = t.phase == 0 && g.tall, q_mn = t.phase == 0 ? g.tall : (t.phase == 2 && !g.tall);
       const int kblocks = t.phase == 0 ? kb_x : kb_k;
       for (int seg = 0; seg < SEGS && ok; ++seg) {
         // hi lo, lo hi, hi hi: the small partial products first
         const int p_lo = (SPLIT && seg == 1) ? 1 : 0, q_lo = (SPLIT && seg == 0) ? 1 : 0;
-        const CUtensorMap* mp = t.phase == 0 ? &g.x_gram[cur][p_lo]
-                                             : (t.phase == 1 ? &g.a_load[p_lo] : (g.tall ? &g.x_apply[cur][p_lo] : &g.b_load[p_lo]));
-        const CUtensorMap* mq = t.phase == 0 ? &g.x_gram[cur][q_lo]
-                                             : (t.phase == 1 ? &g.a_load[q_lo] : (g.tall ? &g.b_load[q_lo] : &g.x_apply[cur][q_lo]));
+        const bool once = t.phase != 2 && t.mb == t.nb && p_lo == q_lo;      // both operands are the same rows
+        // the symmetric factor (A, or B) and, but for B = b A + c A A, the X operand
+        const CUtensorMap* fp = t.phase == 1 ? g.a_load[p_lo] : g.b_load[p_lo];
+        const CUtensorMap* fq = t.phase == 1 ? g.a_load[q_lo] : g.b_load[q_lo];
+        const CUtensorMap* xp = t.phase == 0 ? &g.x_gram[cur][p_lo] : &g.x_apply[cur][p_lo];
+        const CUtensorMap* xq = t.phase == 0 ? &g.x_gram[cur][q_lo] : &g.x_apply[cur][q_lo];
         for (int kb = 0, kx = 0; kb < kblocks; ++kb, kx += NS_BK) {
           if (!__all_sync(0xffffffffu, ns_wait(empty0 + 8 * s, ph ^ 1))) {
             if (lane == 0) ns_abort(bars, status, STATUS_TIMEOUT_SMEM_EMPTY, 80, s);
@@ -325,20 +304,35 @@ __device__ __forceinline__ void ns_chain_body(const NsPlan& g, Status* status) {
           const uint32_t full = full_lead0 + 8 * s;
           const uint32_t p_dst = smem0 + s * NS_STAGE_BYTES, q_dst = p_dst + NS_OPERAND_BYTES;
           if (elect_one()) {
-            if (!PAIR || rank == 0) mbar_arrive_expect_tx(full0 + 8 * s, (PAIR ? 2 : 1) * NS_STAGE_BYTES);
-            auto load = [&](uint32_t dst, const CUtensorMap* m, int x, int y) {
-              if (PAIR) tma_load_3d_pair(dst, m, full, x, y, t.z);
-              else tma_load_3d(dst, m, full, x, y, t.z);
+            if (!PAIR || rank == 0) mbar_arrive_expect_tx(full0 + 8 * s, (PAIR ? 2 : 1) * (once ? NS_OPERAND_BYTES : NS_STAGE_BYTES));
+            auto load = [&](uint32_t dst, const CUtensorMap* m, bool mn, int row) {      // rows row .. row + 127, this K block
+              auto copy = [&](uint32_t d, int x, int y) {
+                if (PAIR) tma_load_3d_pair(d, m, full, x, y, t.z);
+                else tma_load_3d(d, m, full, x, y, t.z);
+              };
+              if (!mn) {
+                copy(dst, kx, row);
+              } else {
+#pragma unroll
+                for (int i = 0; i < 2; ++i) copy(dst + i * (NS_BK * 128), row + i * 64, kx);
+              }
             };
-            if (!p_mn) load(p_dst, mp, kx, m0);
-            else {
-#pragma unroll
-              for (int i = 0; i < 2; ++i) load(p_dst + i * (NS_BK * 128), mp, m0 + i * 64, kx);
-            }
-            if (!q_mn) load(q_dst, mq, kx, n0);
-            else {
-#pragma unroll
-              for (int i = 0; i < 2; ++i) load(q_dst + i * (NS_BK * 128), mq, n0 + i * 64, kx);
+            auto factor = [&](uint32_t dst, const CUtensorMap* m, int block, int row) {
+              const bool mn = ns_below<TILE>(kb, block);
+              load(dst, &m[mn], mn, row);
+            };
+            if (t.phase == 0) {
+              load(p_dst, xp, g.tall, m0);
+              if (!once) load(q_dst, xq, g.tall, n0);
+            } else if (t.phase == 1) {
+              factor(p_dst, fp, t.mb, m0);
+              if (!once) factor(q_dst, fq, t.nb, n0);
+            } else if (g.tall) {
+              load(p_dst, xp, false, m0);
+              factor(q_dst, fq, t.nb, n0);
+            } else {
+              factor(p_dst, fp, t.mb, m0);
+              load(q_dst, xq, true, n0);
             }
           }
           __syncwarp();
@@ -355,14 +349,10 @@ __device__ __forceinline__ void ns_chain_body(const NsPlan& g, Status* status) {
         const int item = ns_next_item(bars, it, status);
         if (item < 0) break;
         const NsItem t = ns_decode(g, item, WARPS_PER_TILE);
-        const bool p_mn = t.phase == 0 && g.tall, q_mn = t.phase == 0 ? g.tall : (t.phase == 2 && !g.tall);
-        const uint32_t idesc = make_instr_desc(0, 0, p_mn ? 1 : 0, q_mn ? 1 : 0, TILE, TILE);
-        const uint32_t p_step = p_mn ? (16 * 128) >> 4 : 2, q_step = q_mn ? (16 * 128) >> 4 : 2;
-        const uint64_t p_tmpl = make_smem_desc(smem0, p_mn ? NS_BK * 128 : 16, 1024);
-        const uint64_t q_tmpl = make_smem_desc(smem0 + NS_OPERAND_BYTES, q_mn ? NS_BK * 128 : 16, 1024);
-        const uint32_t p_hi = (uint32_t)(p_tmpl >> 32), p_lo0 = (uint32_t)p_tmpl;
-        const uint32_t q_hi = (uint32_t)(q_tmpl >> 32), q_lo0 = (uint32_t)q_tmpl;
-        const int blocks = (t.phase == 0 ? kb_x : kb_k) * SEGS;
+        const int kblocks = t.phase == 0 ? kb_x : kb_k;
+        const bool diagonal = t.phase != 2 && t.mb == t.nb;
+        const uint64_t k_tmpl = make_smem_desc(smem0, 16, 1024), mn_tmpl = make_smem_desc(smem0, NS_BK * 128, 1024);
+        const int blocks = kblocks * SEGS;
         // K blocks that one accumulator takes: all of them, or, with pairs, few enough for the sum to stay as exact as fp32
         const int per_acc = SPLIT ? NS_SPLIT_KBLOCKS : blocks;
         for (int b0 = 0; b0 < blocks && ok; b0 += per_acc) {
@@ -375,6 +365,7 @@ __device__ __forceinline__ void ns_chain_body(const NsPlan& g, Status* status) {
           const uint32_t d_tmem = tmem_base + acc * TILE;
           const int count = min(per_acc, blocks - b0);
           uint32_t accumulate = 0;
+          int kb = b0 % kblocks;
           for (int i = 0; i < count; ++i) {
             if (!__all_sync(0xffffffffu, ns_wait(full0 + 8 * s, ph))) {
               if (lane == 0) ns_abort(bars, status, STATUS_TIMEOUT_SMEM_FULL, 82, s);
@@ -382,7 +373,17 @@ __device__ __forceinline__ void ns_chain_body(const NsPlan& g, Status* status) {
               break;
             }
             tc_fence_after_sync();
-            const uint32_t p_lo = p_lo0 + s * (NS_STAGE_BYTES >> 4), q_lo = q_lo0 + s * (NS_STAGE_BYTES >> 4);
+            // major order of this K block's operands
+            const bool p_mn = t.phase == 0 ? g.tall : (t.phase == 1 || !g.tall) && ns_below<TILE>(kb, t.mb);
+            const bool q_mn = t.phase == 0 ? g.tall : (t.phase == 2 && !g.tall) || ns_below<TILE>(kb, t.nb);
+            const uint32_t idesc = make_instr_desc(0, 0, p_mn ? 1 : 0, q_mn ? 1 : 0, TILE, TILE);
+            const uint32_t p_step = p_mn ? (16 * 128) >> 4 : 2, q_step = q_mn ? (16 * 128) >> 4 : 2;
+            const bool once = diagonal && (!SPLIT || b0 + i >= 2 * kblocks);     // hi hi comes last
+            const uint64_t p_tmpl = p_mn ? mn_tmpl : k_tmpl, q_tmpl = q_mn ? mn_tmpl : k_tmpl;
+            const uint32_t p_hi = (uint32_t)(p_tmpl >> 32), q_hi = (uint32_t)(q_tmpl >> 32);
+            const uint32_t p_lo = (uint32_t)p_tmpl + s * (NS_STAGE_BYTES >> 4);
+            const uint32_t q_lo = (uint32_t)q_tmpl + s * (NS_STAGE_BYTES >> 4) + (once ? 0 : NS_OPERAND_BYTES >> 4);
+            if (++kb == kblocks) kb = 0;
             if (elect_one()) {
 #pragma unroll
               for (int k = 0; k < NS_BK / 16; ++k) {
@@ -408,54 +409,88 @@ __device__ __forceinline__ void ns_chain_body(const NsPlan& g, Status* status) {
         }
       }
     }
+  } else if (warp == 2 + NS_EPI_WARPS) {
+    if (rank == 0) {
+      const uint32_t peer_item0 = PAIR ? map_to_cta(smem_u32(&bars->item[0]), 1) : 0;
+      const uint32_t peer_bar0 = PAIR ? map_to_cta(smem_u32(&bars->item_full[0]), 1) : 0;
+      int ahead = lane == 0 ? (int)atomicAdd(g.next_item, 1u) : 0;
+      for (int it = 0;; ++it) {
+        int item = __shfl_sync(0xffffffffu, ahead, 0);
+        if (item >= g.items) item = -1;
+        if (lane == 0) {
+          if (item >= 0) {
+            ahead = (int)atomicAdd(g.next_item, 1u);      // needed one item later
+            const NsItem t = ns_decode(g, item, WARPS_PER_TILE);
+            if (t.need != 0 && !wait_flag_ge_gpu(g.done + t.z, t.need, GD_WAIT_BUDGET_NS)) {
+              ns_abort(bars, status, STATUS_TIMEOUT_PEER_FLAG, 84, t.z);
+              item = -1;
+            }
+            if (it >= 2 && !ns_wait(smem_u32(&bars->taken[it & 1]), ((it >> 1) - 1) & 1)) {
+              if (!ns_aborted(bars)) ns_abort(bars, status, STATUS_TIMEOUT_SMEM_EMPTY, 85, it);
+              item = -1;
+            }
+            if (ns_aborted(bars)) item = -1;
+          }
+          const int slot = it & (NS_RING - 1);
+          *((volatile int*)&bars->item[slot]) = item;
+          mbar_arrive(smem_u32(&bars->item_full[slot]));
+          if (PAIR) {
+            ns_put_remote(peer_item0 + 4 * slot, item);
+            ns_arrive_remote(peer_bar0 + 8 * slot);
+          }
+        }
+        item = __shfl_sync(0xffffffffu, item, 0);
+        if (item < 0) break;
+      }
+    }
   } else {
     const int ew = warp - 2;
-    uint8_t* my_boxes = boxes + ew * NsShape<SPLIT>::WARP_BYTES;
+    uint8_t* aux_slots = boxes + ew * NsShape<SPLIT>::WARP_BYTES;
+    uint8_t* out_box = aux_slots + NS_SLOTS * NsShape<SPLIT>::AUX_BYTES;
     const uint32_t aux_bar0 = smem_u32(&bars->aux_full[ew * NS_SLOTS]);
     const int quarter = warp & 3, half = ew >> 2;
     const uint32_t aempty_lead0 = PAIR ? map_to_cta(aempty0, 0) : aempty0;
     int acc = 0;
     uint32_t acc_ph = 0, aux_ph = 0;             // aux_ph: bit s = phase of slot s
     bool ok = true;
-    for (int it = 0; ok; ++it) {
-      const int item = ns_next_item(bars, it, status);
-      if (item < 0) break;
-      const NsItem t = ns_decode(g, item, WARPS_PER_TILE);
-      const int cur = t.step & 1;
+
+    NsItem t;
+    int m_warp, n_half, chunks;                  // this warp's corner of the tile; chunks that hold anything of the matrix
+    auto take = [&](int item) {
+      t = ns_decode(g, item, WARPS_PER_TILE);
       const int M = t.phase == 2 ? g.rows : g.k, N = t.phase == 2 ? g.cols : g.k;
-      const int m_warp = t.mb * TILE + (int)rank * 128 + quarter * 32;
-      const int n_half = t.nb * TILE + half * (TILE / 2);
-      const bool mirror = t.phase != 2 && t.mb != t.nb;
-      const CUtensorMap* out = t.phase == 0 ? g.a_box : (t.phase == 1 ? g.b_box : g.x_box[cur ^ 1]);
-      const CUtensorMap* aux = t.phase == 1 ? g.a_box : g.x_box[cur];
-      const bool aux_lo = SPLIT || t.phase == 2, store_lo = aux_lo;
-      const float aux_scale = t.phase == 1 ? g.b : g.a, acc_scale = (t.phase == 1 ? g.c : 1.0f) * NS_UNSCALE;
-      // chunks that hold anything of the matrix: the others are not read, computed or stored
-      const int chunks = m_warp < M ? max(0, min(CHUNKS, (N - n_half + 31) / 32)) : 0;
-
-      // the slot is free once its last bulk store has been read; then the linear term's boxes land in it
-      auto aux_request = [&](int c) {
-        if (elect_one()) {
-          bulk_wait_read_all();
-          const int sl = c & (NS_SLOTS - 1);
-          const uint32_t bar = aux_bar0 + 8 * sl, dst = smem_u32(my_boxes) + sl * (SLOT_BOXES * NS_BOX_BYTES);
-          mbar_arrive_expect_tx(bar, (aux_lo ? 2 : 1) * NS_BOX_BYTES);
-          tma_load_3d(dst, &aux[0], bar, n_half + c * 32, m_warp, t.z);
-          if (aux_lo) tma_load_3d(dst + NS_BOX_BYTES, &aux[1], bar, n_half + c * 32, m_warp, t.z);
-        }
-        __syncwarp();
-      };
-      if (t.phase != 0 && chunks > 0) {
-        uint32_t ready = 1;
-        if (lane == 0) ready = wait_flag_ge_gpu(g.done + t.z, t.need, GD_WAIT_BUDGET_NS);
-        if (!__shfl_sync(0xffffffffu, ready, 0)) {
-          ns_abort(bars, status, STATUS_TIMEOUT_PEER_FLAG, 85, t.z);
-          break;
-        }
-        fence_proxy_async_global();
-        for (int c = 0; c < min(chunks, NS_SLOTS); ++c) aux_request(c);
+      m_warp = t.mb * TILE + (int)rank * 128 + quarter * 32;
+      n_half = t.nb * TILE + half * (TILE / 2);
+      chunks = m_warp < M ? max(0, min(CHUNKS, (N - n_half + 31) / 32)) : 0;
+    };
+    // chunk c of the linear term (the old X, or A) into its slot, which every lane has finished reading
+    auto aux_request = [&](int c) {
+      if (elect_one()) {
+        const CUtensorMap* aux = t.phase == 1 ? g.a_box : g.x_box[t.step & 1];
+        const bool lo = SPLIT || t.phase == 2;
+        const int sl = c & (NS_SLOTS - 1);
+        const uint32_t bar = aux_bar0 + 8 * sl, dst = smem_u32(aux_slots) + sl * NsShape<SPLIT>::AUX_BYTES;
+        mbar_arrive_expect_tx(bar, (lo ? 2 : 1) * NS_BOX_BYTES);
+        tma_load_3d(dst, &aux[0], bar, n_half + c * 32, m_warp, t.z);
+        if (lo) tma_load_3d(dst + NS_BOX_BYTES, &aux[1], bar, n_half + c * 32, m_warp, t.z);
       }
+      __syncwarp();
+    };
+    auto aux_begin = [&]() {
+      if (t.phase == 0) return;
+      fence_proxy_async_global();      // the item was handed out after what it reads was written
+      for (int c = 0; c < min(chunks, NS_SLOTS); ++c) aux_request(c);
+    };
 
+    int item = ns_next_item(bars, 0, status);
+    if (item >= 0) {
+      take(item);
+      aux_begin();
+    }
+    for (int it = 0; item >= 0 && ok; ++it) {
+      const CUtensorMap* out = t.phase == 0 ? g.a_box : (t.phase == 1 ? g.b_box : g.x_box[(t.step & 1) ^ 1]);
+      const bool with_lo = SPLIT || t.phase == 2;
+      const float aux_scale = t.phase == 1 ? g.b : g.a, acc_scale = (t.phase == 1 ? g.c : 1.0f) * NS_UNSCALE;
       auto acc_wait = [&]() -> bool {
         if (mbar_wait_warp(afull0 + 8 * acc, acc_ph)) {
           tc_fence_after_sync();
@@ -474,14 +509,78 @@ __device__ __forceinline__ void ns_chain_body(const NsPlan& g, Status* status) {
         if (++acc == NS_ACC) { acc = 0; acc_ph ^= 1; }
       };
       auto acc_row = [&]() { return tmem_base + ((uint32_t)(quarter * 32) << 16) + acc * TILE + half * (TILE / 2); };
-      // Pairs: the tensor core cuts a running sum where fp32 rounds it, an error of one sign that grows with the number of
-      // additions, so every few K blocks the sum moves to registers and is continued there.
-      float sum[SPLIT ? CHUNKS : 1][32];
-      if (SPLIT) {
+
+      // one 32 x 32 chunk: linear term, result as hi + lo, out. `ready` waits for the accumulator values in `raw`
+      auto do_chunk = [&](int c, uint32_t (&raw)[32], auto ready) {
+        float v[32];
+        if (t.phase != 0) {
+          const int sl = c & (NS_SLOTS - 1);
+          if (!mbar_wait_warp(aux_bar0 + 8 * sl, (aux_ph >> sl) & 1)) {
+            ns_abort(bars, status, STATUS_TIMEOUT_SMEM_FULL, 86, ew);
+            ok = false;
+            return;
+          }
+          aux_ph ^= 1u << sl;
+          const uint8_t* slot = aux_slots + sl * NsShape<SPLIT>::AUX_BYTES;
+          uint32_t w[16];
+          ns_read_row(slot, lane, w);
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const float2 f = unpack_half2(w[i]);
+            v[2 * i] = f.x; v[2 * i + 1] = f.y;
+          }
+          if (with_lo) {
+            ns_read_row(slot + NS_BOX_BYTES, lane, w);
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+              const float2 f = unpack_half2(w[i]);
+              v[2 * i] += f.x; v[2 * i + 1] += f.y;
+            }
+          }
+          __syncwarp();
+          if (c + NS_SLOTS < chunks) aux_request(c + NS_SLOTS);
+          ready();
+#pragma unroll
+          for (int j = 0; j < 32; ++j) v[j] = fmaf(aux_scale, v[j], acc_scale * __uint_as_float(raw[j]));
+        } else {
+          ready();
+#pragma unroll
+          for (int j = 0; j < 32; ++j) v[j] = acc_scale * __uint_as_float(raw[j]);
+        }
+        uint32_t hi[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) hi[i] = pack_half2(v[2 * i], v[2 * i + 1]);
+        if (elect_one()) bulk_wait_read_all();      // the stores of the chunk before have left the boxes
+        __syncwarp();
+        ns_write_row(out_box, lane, hi);
+        if (with_lo) {
+          uint32_t lo[16];
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            const float2 h = unpack_half2(hi[i]);
+            lo[i] = pack_half2(v[2 * i] - h.x, v[2 * i + 1] - h.y);
+          }
+          ns_write_row(out_box + NS_BOX_BYTES, lane, lo);
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (elect_one()) {
+          const int n0 = n_half + c * 32;
+          tma_store_3d(&out[0], smem_u32(out_box), n0, m_warp, t.z);
+          if (with_lo) tma_store_3d(&out[1], smem_u32(out_box + NS_BOX_BYTES), n0, m_warp, t.z);
+          bulk_commit_group();
+        }
+        __syncwarp();
+      };
+
+      if constexpr (SPLIT) {
+        // Pairs: the tensor core cuts a running sum where fp32 rounds it, an error of one sign that grows with the number of
+        // additions, so every few K blocks the sum moves to registers and is continued there.
+        float sum[CHUNKS][32];
 #pragma unroll
         for (int c = 0; c < CHUNKS; ++c)
 #pragma unroll
-          for (int j = 0; j < 32; ++j) sum[SPLIT ? c : 0][j] = 0.0f;
+          for (int j = 0; j < 32; ++j) sum[c][j] = 0.0f;
         const int blocks = (t.phase == 0 ? kb_x : kb_k) * SEGS;
         for (int b0 = 0; b0 < blocks && ok; b0 += NS_SPLIT_KBLOCKS) {
           if (!(ok = acc_wait())) break;
@@ -491,109 +590,64 @@ __device__ __forceinline__ void ns_chain_body(const NsPlan& g, Status* status) {
             tmem_ld_32x32(acc_row() + c * 32, raw);
             tmem_ld_wait();
 #pragma unroll
-            for (int j = 0; j < 32; ++j) sum[SPLIT ? c : 0][j] += __uint_as_float(raw[j]);
+            for (int j = 0; j < 32; ++j) sum[c][j] += __uint_as_float(raw[j]);
           }
           acc_release();
         }
-        if (!ok) break;
-      } else {
-        if (!(ok = acc_wait())) break;
-        if (chunks == 0) acc_release();
-      }
-      auto do_chunk = [&](int c, uint32_t (&raw)[32]) {
-        const int sl = c & (NS_SLOTS - 1);
-        uint8_t* slot = my_boxes + sl * (SLOT_BOXES * NS_BOX_BYTES);
-        float aux_v[32];
-        if (t.phase != 0) {
-          if (!mbar_wait_warp(aux_bar0 + 8 * sl, (aux_ph >> sl) & 1)) {
-            ns_abort(bars, status, STATUS_TIMEOUT_SMEM_FULL, 86, ew);
-            ok = false;
-            return;
-          }
-          aux_ph ^= 1u << sl;
-          uint32_t w[16];
-          ns_read_row(slot, lane, w);
-#pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            const float2 f = unpack_half2(w[i]);
-            aux_v[2 * i] = f.x; aux_v[2 * i + 1] = f.y;
-          }
-          if (aux_lo) {
-            ns_read_row(slot + NS_BOX_BYTES, lane, w);
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-              const float2 f = unpack_half2(w[i]);
-              aux_v[2 * i] += f.x; aux_v[2 * i + 1] += f.y;
-            }
-          }
-        } else {
-#pragma unroll
-          for (int j = 0; j < 32; ++j) aux_v[j] = 0.0f;
-          if (elect_one()) bulk_wait_read_but_one();      // the store that used this slot two chunks ago
-          __syncwarp();
-        }
-        if (!SPLIT) {
-          tmem_ld_wait();
-          if (c == chunks - 1) acc_release();
-        }
-        uint32_t hi[16], lo[16];
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const float v0 = fmaf(aux_scale, aux_v[2 * i], acc_scale * __uint_as_float(raw[2 * i]));
-          const float v1 = fmaf(aux_scale, aux_v[2 * i + 1], acc_scale * __uint_as_float(raw[2 * i + 1]));
-          hi[i] = pack_half2(v0, v1);
-          const float2 h = unpack_half2(hi[i]);
-          lo[i] = pack_half2(v0 - h.x, v1 - h.y);
-        }
-        __syncwarp();      // every lane has read its rows of the slot
-        uint8_t* box_t = slot + (SPLIT ? 2 : 1) * NS_BOX_BYTES;
-        ns_write_row(slot, lane, hi);
-        if (store_lo) ns_write_row(slot + NS_BOX_BYTES, lane, lo);
-        if (mirror) {
-          ns_write_transposed(box_t, lane, hi);
-          if (SPLIT) ns_write_transposed(box_t + NS_BOX_BYTES, lane, lo);
-        }
-        fence_proxy_async_smem();
-        __syncwarp();
-        if (elect_one()) {
-          const int n0 = n_half + c * 32;
-          tma_store_3d(&out[0], smem_u32(slot), n0, m_warp, t.z);
-          if (store_lo) tma_store_3d(&out[1], smem_u32(slot + NS_BOX_BYTES), n0, m_warp, t.z);
-          if (mirror) {
-            tma_store_3d(&out[0], smem_u32(box_t), m_warp, n0, t.z);
-            if (SPLIT) tma_store_3d(&out[1], smem_u32(box_t + NS_BOX_BYTES), m_warp, n0, t.z);
-          }
-          bulk_commit_group();
-        }
-        __syncwarp();
-        if (t.phase != 0 && c + NS_SLOTS < chunks) aux_request(c + NS_SLOTS);
-      };
-      if constexpr (SPLIT) {
 #pragma unroll
         for (int c = 0; c < CHUNKS; ++c) {
           if (c >= chunks || !ok) continue;
           uint32_t raw[32];
 #pragma unroll
           for (int j = 0; j < 32; ++j) raw[j] = __float_as_uint(sum[c][j]);
-          do_chunk(c, raw);
+          do_chunk(c, raw, []() {});
         }
       } else {
+        if (!(ok = acc_wait())) break;
+        if (chunks == 0) acc_release();
+        // two register buffers: the accumulator's next chunk is on its way while this one is worked on
+        uint32_t raw0[32], raw1[32];
+        if (chunks > 0) tmem_ld_32x32(acc_row(), raw0);
 #pragma unroll 1
-        for (int c = 0; c < chunks && ok; ++c) {
-          uint32_t raw[32];
-          tmem_ld_32x32(acc_row() + c * 32, raw);
-          do_chunk(c, raw);
+        for (int c = 0; c < chunks && ok; c += 2) {
+          do_chunk(c, raw0, [&]() {
+            tmem_ld_wait();
+            if (c + 1 < chunks) tmem_ld_32x32(acc_row() + (c + 1) * 32, raw1);
+            else acc_release();
+          });
+          if (c + 1 >= chunks || !ok) break;
+          do_chunk(c + 1, raw1, [&]() {
+            tmem_ld_wait();
+            if (c + 2 < chunks) tmem_ld_32x32(acc_row() + (c + 2) * 32, raw0);
+            else acc_release();
+          });
         }
       }
       if (!ok) break;
-      // this warp's part of the tile is written: count it
-      if (elect_one()) {
+      // The next item's linear term can be asked for before this one's stores are complete, but not waited for: what
+      // it reads may depend on the count below.
+      const int z_done = t.z;
+      const bool there = ns_item_there(bars, it + 1);
+      if (there) {
+        item = ns_next_item(bars, it + 1, status);
+        if (item >= 0) {
+          take(item);
+          aux_begin();
+        }
+      }
+      if (elect_one()) {               // this warp's part of the tile is written: count it
         bulk_wait_all();
         fence_proxy_async_global();
-        __threadfence();
-        asm volatile("red.release.gpu.global.add.u32 [%0], 1;" ::"l"(g.done + t.z) : "memory");
+        asm volatile("red.release.gpu.global.add.u32 [%0], 1;" ::"l"(g.done + z_done) : "memory");
       }
       __syncwarp();
+      if (!there) {
+        item = ns_next_item(bars, it + 1, status);
+        if (item >= 0) {
+          take(item);
+          aux_begin();
+        }
+      }
     }
     if (elect_one()) bulk_wait_all();
     __syncwarp();
@@ -911,9 +965,8 @@ const char* launch_orthogonalize(const NsCall& call, Status* status, cudaStream_
   uint8_t* tail = reinterpret_cast<uint8_t*>(call.workspace) + 2 * w.partial;
   const bool tall = rows > cols;
 
-  int dev = 0, sms = 0, l2 = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess ||
-      cudaDeviceGetAttribute(&l2, cudaDevAttrL2CacheSize, dev) != cudaSuccess)
+  int dev = 0, sms = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
     return "orthogonalize: device";
 
   NsPlan g;
@@ -965,12 +1018,6 @@ const char* launch_orthogonalize(const NsCall& call, Status* status, cudaStream_
   g.tiles_x = kt * wt;
   g.tiles_xm = tall ? wt : kt;
   const int units = pair ? sms / 2 : sms;
-  // as many matrices as L2 holds with their two X buffers, A and B, but enough tiles to keep every unit busy twice
-  const int64_t bytes = 2 * (w.x * 2 + w.k * (call.pairs ? 2 : 1)) / batch;
-  int64_t window = l2 / bytes;
-  const int64_t least = (2 * units + g.tiles_sym - 1) / g.tiles_sym;
-  if (window < least) window = least;
-  g.window = (int)(window < batch ? window : batch);
   const int64_t items = batch * g.steps * (2 * g.tiles_sym + g.tiles_x);
   if (items > (1ll << 30)) return "orthogonalize: too many tiles";
   g.items = (int)items;
@@ -989,8 +1036,10 @@ const char* launch_orthogonalize(const NsCall& call, Status* status, cudaStream_
       load_map(&g.x_apply[i][lo], p, rows, cols, w.ld_x, w.plane_x, !tall);    // B X: X is the MN-major second operand; tall: X B^T
       box_map(&g.x_box[i][lo], p, rows, cols, w.ld_x, w.plane_x);
     }
-    load_map(&g.a_load[lo], A + lo * lo_k, g.k, g.k, w.ld_k, w.plane_k, false);
-    load_map(&g.b_load[lo], B + lo * lo_k, g.k, g.k, w.ld_k, w.plane_k, false);
+    for (int mn = 0; mn < 2; ++mn) {
+      load_map(&g.a_load[lo][mn], A + lo * lo_k, g.k, g.k, w.ld_k, w.plane_k, mn);
+      load_map(&g.b_load[lo][mn], B + lo * lo_k, g.k, g.k, w.ld_k, w.plane_k, mn);
+    }
     box_map(&g.a_box[lo], A + lo * lo_k, g.k, g.k, w.ld_k, w.plane_k);
     box_map(&g.b_box[lo], B + lo * lo_k, g.k, g.k, w.ld_k, w.plane_k);
   }

@@ -36,14 +36,14 @@ struct NsEnds {
   uint32_t* next_item;
 };
 
-// All products of a call (see ns_chain_body). Tensor maps [buffer][hi, lo].
+// All products of a call (see ns_chain_body). Tensor maps [buffer][hi, lo], of the symmetric factors [hi, lo][K-major, MN-major].
 struct NsPlan {
   CUtensorMap x_gram[2][2], x_apply[2][2], x_box[2][2];
-  CUtensorMap a_load[2], a_box[2], b_load[2], b_box[2];
+  CUtensorMap a_load[2][2], b_load[2][2], a_box[2], b_box[2];
   int batch, steps, rows, cols, tall;
   int k, wide;                         // smaller and larger side
   int tiles_sym, tiles_x, tiles_xm;    // tiles of a symmetric product, of X, row blocks of X
-  int window, items;
+  int items;
   float a, b, c;
   uint32_t* done;                      // [batch] finished tiles, counted in epilogue warps
   uint32_t* next_item;
