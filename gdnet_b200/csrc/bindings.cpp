@@ -1171,7 +1171,7 @@ void orthogonalize(const Tensor& x, Tensor out, int64_t steps, at::ArrayRef<doub
   call.ends.out_dtype = elem_type(out, "out");
   call.ends.grad_ld = x.stride(1);
   const int64_t group = ns_group(n, rows, cols);
-  Tensor space = at::empty({gd::ns_workspace_bytes(group, rows, cols)}, x.options().dtype(at::kByte));
+  Tensor space = at::empty({gd::ns_workspace_bytes(group, rows, cols, call.steps, call.pairs)}, x.options().dtype(at::kByte));
   call.workspace = space.data_ptr();
   for (int64_t i0 = 0; i0 < n; i0 += group) {
     const int64_t count = std::min(group, n - i0);
@@ -1220,7 +1220,7 @@ void muon_update(at::TensorList params, at::TensorList grads, at::TensorList inf
   call.ends.decay = (float)decay;
   call.ends.step = (float)step;
   const int64_t group = ns_group(n, rows, cols);
-  Tensor space = at::empty({gd::ns_workspace_bytes(group, rows, cols)}, first.options().dtype(at::kByte));
+  Tensor space = at::empty({gd::ns_workspace_bytes(group, rows, cols, call.steps, call.pairs)}, first.options().dtype(at::kByte));
   call.workspace = space.data_ptr();
   for (int64_t i0 = 0; i0 < n; i0 += group) {
     const int64_t count = std::min(group, n - i0);

@@ -91,7 +91,7 @@ struct NsShape {
   static constexpr int SMEM = STAGES * NS_STAGE_BYTES + NS_EPI_WARPS * WARP_BYTES + 1024 + 1024;   // barriers; alignment
 };
 
-struct __align__(8) NsBars {
+struct __align__(16) NsBars {
   uint64_t full[4];
   uint64_t empty[4];
   uint64_t acc_full[NS_ACC];
@@ -99,11 +99,12 @@ struct __align__(8) NsBars {
   uint64_t aux_full[NS_EPI_WARPS * NS_SLOTS];
   uint64_t item_full[NS_RING];
   uint64_t taken[2];                 // the loads have begun item it (barrier it & 1)
-  int item[NS_RING];
+  uint4 item[NS_RING];               // see NsItem::pack
   uint32_t tmem_base;
   int abort;
 };
 static_assert(sizeof(NsBars) <= 1024, "barrier area");
+constexpr int NS_MAPS = 24;                     // tensor maps at the start of NsPlan
 
 __device__ __forceinline__ bool ns_aborted(const NsBars* b) { return *((volatile const int*)&b->abort) != 0; }
 __device__ __forceinline__ void ns_abort(NsBars* b, Status* st, int code, int site, int detail) {
@@ -128,20 +129,27 @@ __device__ __forceinline__ uint32_t ns_try_wait_cluster(uint32_t bar, uint32_t p
       : "memory");
   return ok;
 }
-__device__ __forceinline__ void ns_put_remote(uint32_t cluster_addr, int v) {
-  asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(cluster_addr), "r"(v) : "memory");
+__device__ __forceinline__ void ns_put_remote(uint32_t cluster_addr, uint4 v) {
+  asm volatile("st.shared::cluster.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(cluster_addr), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
 }
 __device__ __forceinline__ void ns_arrive_remote(uint32_t cluster_bar) {
   asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_bar) : "memory");
 }
 
-// Item `slot_no` of this block's list, -1 at its end or when the wait ran out. Warp-collective.
-__device__ __forceinline__ int ns_next_item(NsBars* bars, int slot_no, Status* status) {
+struct NsItem {
+  int live;                          // 0: the list has ended
+  int step, phase, z, mb, nb;        // phase 0: A, 1: B, 2: X
+  __device__ __forceinline__ uint4 pack() const {
+    return make_uint4((uint32_t)z, (uint32_t)(step | phase << 16), (uint32_t)mb, (uint32_t)nb | (uint32_t)live << 31);
+  }
+};
+
+// Item `slot_no` of this block's list; not live at its end or when the wait ran out. Warp-collective.
+__device__ __forceinline__ NsItem ns_next_item(NsBars* bars, int slot_no, Status* status) {
   const uint32_t bar = smem_u32(&bars->item_full[slot_no & (NS_RING - 1)]);
   const uint32_t parity = (slot_no / NS_RING) & 1;
-  int item = -1;
+  bool ok = false;
   if ((threadIdx.x & 31) == 0) {
-    bool ok = false;
     for (int i = 0; i < 256 && !ok; ++i) ok = ns_try_wait_cluster(bar, parity);
     if (!ok) {
       const uint64_t t0 = globaltimer_ns();
@@ -154,9 +162,20 @@ __device__ __forceinline__ int ns_next_item(NsBars* bars, int slot_no, Status* s
         }
       }
     }
-    if (ok) item = *((volatile int*)&bars->item[slot_no & (NS_RING - 1)]);
   }
-  return __shfl_sync(0xffffffffu, item, 0);
+  ok = __shfl_sync(0xffffffffu, ok, 0);
+  NsItem t;
+  t.live = 0;
+  if (!ok) return t;
+  const volatile uint4* at = &bars->item[slot_no & (NS_RING - 1)];
+  const uint32_t x = at->x, y = at->y, m = at->z, n = at->w;
+  t.z = (int)x;
+  t.step = (int)(y & 0xffffu);
+  t.phase = (int)(y >> 16);
+  t.mb = (int)m;
+  t.nb = (int)(n & 0x7fffffffu);
+  t.live = (int)(n >> 31);
+  return t;
 }
 
 // Whether ns_next_item(slot_no) would return at once. Warp-collective.
@@ -167,13 +186,10 @@ __device__ __forceinline__ bool ns_item_there(NsBars* bars, int slot_no) {
   return __shfl_sync(0xffffffffu, ok, 0) != 0;
 }
 
-struct NsItem {
-  int step, phase, z, mb, nb;        // phase 0: A, 1: B, 2: X
-  uint32_t need;                     // finished tiles of matrix z that this one reads (in epilogue warps)
-};
-
-__device__ __forceinline__ NsItem ns_decode(const NsPlan& g, int item, uint32_t warps_per_tile) {
+// `need`: finished tiles of matrix z that this one reads (counted in epilogue warps)
+__device__ __forceinline__ NsItem ns_decode(const NsPlan& g, int item, uint32_t warps_per_tile, uint32_t& need) {
   NsItem t;
+  t.live = 1;
   const int per_step = 2 * g.tiles_sym + g.tiles_x;
   t.step = item / (g.batch * per_step);
   int r = item - t.step * g.batch * per_step;
@@ -184,7 +200,7 @@ __device__ __forceinline__ NsItem ns_decode(const NsPlan& g, int item, uint32_t 
   else if (r >= sym) { t.phase = 1; r -= sym; }
   t.z = r / tiles;
   r -= t.z * tiles;
-  t.need = (uint32_t)(t.step * per_step + t.phase * g.tiles_sym) * warps_per_tile;
+  need = (uint32_t)(t.step * per_step + t.phase * g.tiles_sym) * warps_per_tile;
   if (t.phase == 2) {
     t.nb = r / g.tiles_xm;           // neighbours share a column block
     t.mb = r - t.nb * g.tiles_xm;
@@ -256,6 +272,11 @@ __device__ __forceinline__ void ns_chain_body(const NsPlan& g, Status* status) {
     bars->abort = 0;
     fence_barrier_init();
   }
+  // the tensor maps of the first items are fetched while the block starts
+  if (warp >= 2) {
+    const CUtensorMap* maps = &g.x_gram[0][0];
+    for (int i = (warp - 2) * 32 + lane; i < (int)(NS_MAPS); i += (NS_THREADS - 64)) tma_prefetch_desc(maps + i);
+  }
   if (warp == 1) {
     if (PAIR) { tmem_alloc_pair(smem_u32(&bars->tmem_base), NS_ACC * TILE); tmem_relinquish_pair(); }
     else { tmem_alloc(smem_u32(&bars->tmem_base), NS_ACC * TILE); tmem_relinquish(); }
@@ -278,10 +299,9 @@ __device__ __forceinline__ void ns_chain_body(const NsPlan& g, Status* status) {
     uint32_t ph = 0;
     bool ok = true;
     for (int it = 0; ok; ++it) {
-      const int item = ns_next_item(bars, it, status);
-      if (item < 0) break;
+      const NsItem t = ns_next_item(bars, it, status);
+      if (!t.live) break;
       if (rank == 0 && lane == 0) mbar_arrive(smem_u32(&bars->taken[it & 1]));
-      const NsItem t = ns_decode(g, item, WARPS_PER_TILE);
       fence_proxy_async_global();      // what other blocks wrote before they counted up is read by bulk copies below
       const int cur = t.step & 1;
       const int m0 = t.mb * TILE + (int)rank * 128, n0 = t.nb * TILE + (int)rank * 128;
@@ -346,9 +366,8 @@ __device__ __forceinline__ void ns_chain_body(const NsPlan& g, Status* status) {
       uint32_t ph = 0, acc_ph = 0;
       bool ok = true;
       for (int it = 0; ok; ++it) {
-        const int item = ns_next_item(bars, it, status);
-        if (item < 0) break;
-        const NsItem t = ns_decode(g, item, WARPS_PER_TILE);
+        const NsItem t = ns_next_item(bars, it, status);
+        if (!t.live) break;
         const int kblocks = t.phase == 0 ? kb_x : kb_k;
         const bool diagonal = t.phase != 2 && t.mb == t.nb;
         const uint64_t k_tmpl = make_smem_desc(smem0, 16, 1024), mn_tmpl = make_smem_desc(smem0, NS_BK * 128, 1024);
@@ -413,35 +432,37 @@ __device__ __forceinline__ void ns_chain_body(const NsPlan& g, Status* status) {
     if (rank == 0) {
       const uint32_t peer_item0 = PAIR ? map_to_cta(smem_u32(&bars->item[0]), 1) : 0;
       const uint32_t peer_bar0 = PAIR ? map_to_cta(smem_u32(&bars->item_full[0]), 1) : 0;
-      int ahead = lane == 0 ? (int)atomicAdd(g.next_item, 1u) : 0;
-      for (int it = 0;; ++it) {
-        int item = __shfl_sync(0xffffffffu, ahead, 0);
-        if (item >= g.items) item = -1;
-        if (lane == 0) {
-          if (item >= 0) {
+      if (lane == 0) {
+        int ahead = (int)atomicAdd(g.next_item, 1u);
+        NsItem t{};
+        for (int it = 0;; ++it) {
+          t.live = 0;
+          if (ahead < g.items) {
+            uint32_t need;
+            t = ns_decode(g, ahead, WARPS_PER_TILE, need);
             ahead = (int)atomicAdd(g.next_item, 1u);      // needed one item later
-            const NsItem t = ns_decode(g, item, WARPS_PER_TILE);
-            if (t.need != 0 && !wait_flag_ge_gpu(g.done + t.z, t.need, GD_WAIT_BUDGET_NS)) {
+            if (need != 0 && !wait_flag_ge_gpu(g.done + t.z, need, GD_WAIT_BUDGET_NS)) {
               ns_abort(bars, status, STATUS_TIMEOUT_PEER_FLAG, 84, t.z);
-              item = -1;
+              t.live = 0;
             }
             if (it >= 2 && !ns_wait(smem_u32(&bars->taken[it & 1]), ((it >> 1) - 1) & 1)) {
               if (!ns_aborted(bars)) ns_abort(bars, status, STATUS_TIMEOUT_SMEM_EMPTY, 85, it);
-              item = -1;
+              t.live = 0;
             }
-            if (ns_aborted(bars)) item = -1;
+            if (ns_aborted(bars)) t.live = 0;
           }
           const int slot = it & (NS_RING - 1);
-          *((volatile int*)&bars->item[slot]) = item;
+          const uint4 w = t.pack();
+          bars->item[slot] = w;
           mbar_arrive(smem_u32(&bars->item_full[slot]));
           if (PAIR) {
-            ns_put_remote(peer_item0 + 4 * slot, item);
+            ns_put_remote(peer_item0 + 16 * slot, w);
             ns_arrive_remote(peer_bar0 + 8 * slot);
           }
+          if (!t.live) break;
         }
-        item = __shfl_sync(0xffffffffu, item, 0);
-        if (item < 0) break;
       }
+      __syncwarp();
     }
   } else {
     const int ew = warp - 2;
@@ -454,10 +475,9 @@ __device__ __forceinline__ void ns_chain_body(const NsPlan& g, Status* status) {
     uint32_t acc_ph = 0, aux_ph = 0;             // aux_ph: bit s = phase of slot s
     bool ok = true;
 
-    NsItem t;
+    NsItem t{};
     int m_warp, n_half, chunks;                  // this warp's corner of the tile; chunks that hold anything of the matrix
-    auto take = [&](int item) {
-      t = ns_decode(g, item, WARPS_PER_TILE);
+    auto corner = [&]() {
       const int M = t.phase == 2 ? g.rows : g.k, N = t.phase == 2 ? g.cols : g.k;
       m_warp = t.mb * TILE + (int)rank * 128 + quarter * 32;
       n_half = t.nb * TILE + half * (TILE / 2);
@@ -482,12 +502,12 @@ __device__ __forceinline__ void ns_chain_body(const NsPlan& g, Status* status) {
       for (int c = 0; c < min(chunks, NS_SLOTS); ++c) aux_request(c);
     };
 
-    int item = ns_next_item(bars, 0, status);
-    if (item >= 0) {
-      take(item);
+    t = ns_next_item(bars, 0, status);
+    if (t.live) {
+      corner();
       aux_begin();
     }
-    for (int it = 0; item >= 0 && ok; ++it) {
+    for (int it = 0; t.live && ok; ++it) {
       const CUtensorMap* out = t.phase == 0 ? g.a_box : (t.phase == 1 ? g.b_box : g.x_box[(t.step & 1) ^ 1]);
       const bool with_lo = SPLIT || t.phase == 2;
       const float aux_scale = t.phase == 1 ? g.b : g.a, acc_scale = (t.phase == 1 ? g.c : 1.0f) * NS_UNSCALE;
@@ -629,9 +649,9 @@ __device__ __forceinline__ void ns_chain_body(const NsPlan& g, Status* status) {
       const int z_done = t.z;
       const bool there = ns_item_there(bars, it + 1);
       if (there) {
-        item = ns_next_item(bars, it + 1, status);
-        if (item >= 0) {
-          take(item);
+        t = ns_next_item(bars, it + 1, status);
+        if (t.live) {
+          corner();
           aux_begin();
         }
       }
@@ -642,9 +662,9 @@ __device__ __forceinline__ void ns_chain_body(const NsPlan& g, Status* status) {
       }
       __syncwarp();
       if (!there) {
-        item = ns_next_item(bars, it + 1, status);
-        if (item >= 0) {
-          take(item);
+        t = ns_next_item(bars, it + 1, status);
+        if (t.live) {
+          corner();
           aux_begin();
         }
       }
@@ -747,8 +767,23 @@ __device__ __forceinline__ void add_squares(double& ssq, const VecF<V>& u) {
   }
 }
 
-// u (fp32, row pitch ld) of every matrix and the blocks' partial sums of u^2. Without momentum u is the input itself.
+// u: the gradient, in place the matrix to orthogonalise; f: information gradient; m: momentum, updated
 //   g = scalars[1] * ((1 - beta * scalars[0]) * gt + beta * gi);   m <- mu m + g;   u = nesterov ? g + mu m : m
+template <int V>
+__device__ __forceinline__ void momentum_step(const NsEnds& e, float kt, float ki, bool info, VecF<V>& u, const VecF<V>& f, VecF<V>& m) {
+#pragma unroll
+  for (int i = 0; i < V; ++i) {
+    float x = u.e[i];
+    if (e.scalars != nullptr) {
+      x *= kt;
+      if (info) x = fmaf(ki, f.e[i], x);
+    }
+    m.e[i] = fmaf(e.mu, m.e[i], x);
+    u.e[i] = e.nesterov ? fmaf(e.mu, m.e[i], x) : m.e[i];
+  }
+}
+
+// u (fp32, row pitch ld) of every matrix and the blocks' partial sums of u^2. Without momentum u is the input itself.
 template <int V>
 __global__ void __launch_bounds__(ENDS_THREADS)
 ns_begin_kernel(const __grid_constant__ NsEnds e) {
@@ -789,16 +824,7 @@ ns_begin_kernel(const __grid_constant__ NsEnds e) {
         if (r >= e.rows) continue;
         VecF<V> u = g[q];
         if (e.momentum) {
-#pragma unroll
-          for (int i = 0; i < V; ++i) {
-            float x = g[q].e[i];
-            if (e.scalars != nullptr) {
-              x *= kt;
-              if (gi != nullptr) x = fmaf(ki, f[q].e[i], x);
-            }
-            m[q].e[i] = fmaf(e.mu, m[q].e[i], x);
-            u.e[i] = e.nesterov ? fmaf(e.mu, m[q].e[i], x) : m[q].e[i];
-          }
+          momentum_step<V>(e, kt, ki, gi != nullptr, u, f[q], m[q]);
           *reinterpret_cast<VecF<V>*>(mom + (int64_t)r * e.cols + c) = m[q];
         }
         *reinterpret_cast<VecF<V>*>(up + (int64_t)r * e.ld + c) = u;
@@ -892,6 +918,424 @@ ns_end_kernel(const __grid_constant__ NsEnds e) {
 }
 
 // ---------------------------------------------------------------------------------------
+// matrices with a side of at most 128: a whole call in one kernel
+// ---------------------------------------------------------------------------------------
+// One cluster per matrix; each of its 1 to 16 CTAs keeps a slice of the long side (64 n columns of X, k rows) for the whole call:
+// the fp32 X in TMEM, its fp16 operands in shared memory. A tile of X lies as k rows of 128-byte pieces, which is the K-major
+// operand of A = X X^T and, read as rows of the reduction, the MN-major operand of B X. X in TMEM is stored times a, so that
+// the MMAs of B X add to the linear term in place (with pairs B X has columns of its own and is added in registers: the
+// tensor core cuts a sum where fp32 rounds it, and a X is several times the result). The slices' shares of A are summed through distributed shared memory:
+// every CTA adds up some of the rows, in the order of the CTAs, and hands them to all. What bounds this kernel is the chain of
+// 3 x steps products with an exchange of operands between them (about 2.5 us a step in one CTA), not work or traffic;
+// one 128 x 512 matrix took 111 us as tiles handed out by ns_chain_body.
+constexpr int SM_THREADS = 512;                      // 16 warps: four share the rows of a lane quarter and split its columns
+constexpr int SM_PANEL = 128 * 128;                 // 128 rows x 64 fp16
+constexpr int SM_STAGE_LD = 65;                     // fp32 staging of a panel, one word of padding a row
+
+template <bool SPLIT>
+struct SmShape {
+  static constexpr int SLICE = SPLIT ? 128 : 256;                    // columns a CTA holds at most
+  static constexpr int PLANES = SPLIT ? 2 : 1;                       // hi, lo
+  static constexpr int X_BYTES = SLICE / 64 * SM_PANEL;              // one plane of X
+  static constexpr int F_BYTES = 2 * SM_PANEL;                       // one plane of A or B
+  static constexpr int PART_BYTES = 128 * 128 * 4;                   // this CTA's share of A in fp32
+  // pairs: the shares lie where B does, which is not in use between B X and the next B
+  static constexpr int SMEM = PLANES * (X_BYTES + 2 * F_BYTES) + (SPLIT ? 0 : PART_BYTES) + 1024;
+  static constexpr int X_COL = 0, ACC_COL = SLICE;                   // TMEM columns
+  static constexpr int BX_COL = SPLIT ? SLICE + 128 : X_COL;
+  static constexpr int TMEM_COLS = 512;
+};
+
+__device__ __forceinline__ void tmem_st_32x32(uint32_t taddr, const uint32_t (&v)[32]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31};"
+      ::"r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]),
+        "r"(v[8]), "r"(v[9]), "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]),
+        "r"(v[16]), "r"(v[17]), "r"(v[18]), "r"(v[19]), "r"(v[20]), "r"(v[21]), "r"(v[22]), "r"(v[23]),
+        "r"(v[24]), "r"(v[25]), "r"(v[26]), "r"(v[27]), "r"(v[28]), "r"(v[29]), "r"(v[30]), "r"(v[31]), "r"(taddr)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+__device__ __forceinline__ float4 ld_dsmem_f4(uint32_t addr, uint32_t rank) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w)
+               : "r"(map_to_cta(addr, rank))
+               : "memory");
+  return v;
+}
+__device__ __forceinline__ double ld_dsmem_f64(uint32_t addr, uint32_t rank) {
+  double v;
+  asm volatile("ld.shared::cluster.f64 %0, [%1];" : "=d"(v) : "r"(map_to_cta(addr, rank)) : "memory");
+  return v;
+}
+__device__ __forceinline__ void st_dsmem_u2(uint32_t addr, uint32_t rank, uint2 v) {
+  asm volatile("st.shared::cluster.v2.u32 [%0], {%1, %2};" ::"r"(map_to_cta(addr, rank)), "r"(v.x), "r"(v.y) : "memory");
+}
+
+// byte of (row, 16-byte piece) in a panel: 128-byte rows, pieces XOR-ed with the row
+__device__ __forceinline__ int sm_piece(int row, int piece) { return row * 128 + ((piece ^ (row & 7)) << 4); }
+
+// 32 values of row `row`, columns col .. col + 31 of an operand, as hi (and lo, `plane` bytes further)
+template <bool SPLIT>
+__device__ __forceinline__ void sm_put_operand(uint8_t* base, int plane, int row, int col, const float (&v)[32]) {
+  uint8_t* panel = base + (col >> 6) * SM_PANEL;
+  const int piece0 = (col & 63) >> 3;
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    uint32_t hi[4], lo[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      hi[i] = pack_half2(v[8 * q + 2 * i], v[8 * q + 2 * i + 1]);
+      if (SPLIT) {
+        const float2 h = unpack_half2(hi[i]);
+        lo[i] = pack_half2(v[8 * q + 2 * i] - h.x, v[8 * q + 2 * i + 1] - h.y);
+      }
+    }
+    *reinterpret_cast<uint4*>(panel + sm_piece(row, piece0 + q)) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+    if (SPLIT) *reinterpret_cast<uint4*>(panel + plane + sm_piece(row, piece0 + q)) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+  }
+}
+
+// V elements an access (neighbouring along the memory's rows)
+template <bool SPLIT, int V>
+__global__ void __launch_bounds__(SM_THREADS, 1)
+ns_small_kernel(const __grid_constant__ NsEnds e, const __grid_constant__ NsSmall g, Status* status) {
+  using S = SmShape<SPLIT>;
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ __align__(8) uint64_t bar;
+  __shared__ uint32_t tmem_slot;
+  __shared__ int failed;
+  __shared__ double red[SM_THREADS / 32];
+  __shared__ double ssq_cta;
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* xs = smem;
+  uint8_t* as = xs + S::PLANES * S::X_BYTES;
+  uint8_t* bs = as + S::PLANES * S::F_BYTES;
+  uint8_t* part = SPLIT ? bs : bs + S::F_BYTES;
+  float* staging = reinterpret_cast<float*>(part);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int quarter = warp & 3, part4 = warp >> 2, row = quarter * 32 + lane;
+  const uint32_t ctas = g.ctas, rank = ctas > 1 ? cluster_ctarank() : 0;
+  const int z = blockIdx.x / ctas;
+  const int slice = g.slice, panels = slice >> 6, s0 = (int)rank * slice;
+  const uint32_t mma_bar = smem_u32(&bar);
+
+  if (tid == 0) {
+    mbar_init(mma_bar, 1);
+    failed = 0;
+    fence_barrier_init();
+  }
+  if (warp == 0) {
+    tmem_alloc(smem_u32(&tmem_slot), S::TMEM_COLS);
+    tmem_relinquish();
+  }
+  tc_fence_before_sync();
+  __syncthreads();
+  tc_fence_after_sync();
+  const uint32_t tmem_row = tmem_slot + ((uint32_t)(quarter * 32) << 16);
+  uint32_t phase = 0;
+
+  // ---- the matrix (or the momentum update that makes it) -> TMEM, and its sum of squares
+  float kt = 1.0f, ki = 0.0f;
+  if (e.scalars != nullptr) {
+    kt = (1.0f - e.beta * e.scalars[0]) * e.scalars[1];
+    ki = e.beta * e.scalars[1];
+  }
+  const void* gt = e.grad[z];
+  const void* gi = e.info[z];
+  float* mom = reinterpret_cast<float*>(e.moment[z]);
+  // Element (i, j) of X is element (i, j) of the matrix, or (j, i) of a tall one; neighbouring threads take neighbouring
+  // addresses. Access n of panel p: V elements from (i, j) on, along j (along i when tall).
+  constexpr int ACCESSES = 128 * 64 / V / SM_THREADS, AT_ONCE = ACCESSES < 8 ? ACCESSES : 8;
+  auto coord = [&](int p, int n, int& i, int& j) {
+    const int t = n * SM_THREADS + tid;
+    if (g.tall) { i = t % (128 / V) * V; j = p * 64 + t / (128 / V); }
+    else { i = t / (64 / V); j = p * 64 + t % (64 / V) * V; }
+    return i < g.k && s0 + j < g.wide;
+  };
+  double ssq = 0.0;
+  for (int p = 0; p < panels; ++p) {
+#pragma unroll 1
+    for (int n0 = 0; n0 < ACCESSES; n0 += AT_ONCE) {
+      VecF<V> u[AT_ONCE], f[AT_ONCE], m[AT_ONCE];
+#pragma unroll
+      for (int q = 0; q < AT_ONCE; ++q) {
+        int i, j;
+        if (coord(p, n0 + q, i, j)) {
+          const int64_t r = g.tall ? s0 + j : i, c = g.tall ? i : s0 + j;
+          u[q] = load_vec<V>(gt, e.grad_dtype, r * e.grad_ld + c);
+          if (e.momentum) {
+            m[q] = *reinterpret_cast<const VecF<V>*>(mom + r * e.cols + c);
+            if (gi != nullptr) f[q] = load_vec<V>(gi, e.grad_dtype, r * e.grad_ld + c);
+          }
+        } else {
+#pragma unroll
+          for (int x = 0; x < V; ++x) u[q].e[x] = 0.0f;
+        }
+      }
+#pragma unroll
+      for (int q = 0; q < AT_ONCE; ++q) {
+        int i, j;
+        if (coord(p, n0 + q, i, j) && e.momentum) {
+          const int64_t r = g.tall ? s0 + j : i, c = g.tall ? i : s0 + j;
+          momentum_step<V>(e, kt, ki, gi != nullptr, u[q], f[q], m[q]);
+          *reinterpret_cast<VecF<V>*>(mom + r * e.cols + c) = m[q];
+        }
+#pragma unroll
+        for (int x = 0; x < V; ++x) staging[(i + (g.tall ? x : 0)) * SM_STAGE_LD + (j & 63) + (g.tall ? 0 : x)] = u[q].e[x];
+        add_squares<V>(ssq, u[q]);
+      }
+    }
+    __syncthreads();
+    if (part4 < 2) {
+      uint32_t w[32];
+#pragma unroll
+      for (int c = 0; c < 32; ++c) w[c] = __float_as_uint(staging[row * SM_STAGE_LD + part4 * 32 + c]);
+      tmem_st_32x32(tmem_row + S::X_COL + p * 64 + part4 * 32, w);
+      tmem_st_wait();
+    }
+    __syncthreads();
+  }
+  tc_fence_before_sync();
+  double total = block_sum(ssq, red);
+  if (ctas > 1) {
+    if (tid == 0) ssq_cta = total;
+    cluster_sync_all();
+    total = 0.0;
+    for (uint32_t c = 0; c < ctas; ++c) total += ld_dsmem_f64(smem_u32(&ssq_cta), c);
+  }
+  const double inv = (double)NS_SCALE / (sqrt(total) + (double)e.eps);
+  const float finv = (float)inv;
+  const bool fine = finv > 1e-30f && finv < 1e30f;      // else the factor itself does not fit fp32
+
+  tc_fence_after_sync();
+
+  // all MMAs issued so far are done: their results can be read
+  auto mma_wait = [&]() {
+    if (!*((volatile int*)&failed) && !mbar_wait(mma_bar, phase)) {
+      report(status, STATUS_TIMEOUT_TMEM_FULL, 88, z);
+      *((volatile int*)&failed) = 1;
+    }
+    phase ^= 1;
+    tc_fence_after_sync();
+  };
+  // operands written by all threads (of all CTAs) -> the issuing thread's MMAs
+  auto publish = [&](bool cluster) {
+    fence_proxy_async_smem();
+    tc_fence_before_sync();
+    if (cluster) {
+      asm volatile("fence.proxy.async;" ::: "memory");      // the other CTAs' shared memory as well
+      cluster_sync_all();
+      fence_proxy_async_smem();
+    } else {
+      __syncthreads();
+    }
+    tc_fence_after_sync();
+  };
+  const uint32_t xs_addr = smem_u32(xs), as_addr = smem_u32(as), bs_addr = smem_u32(bs);
+  // acc (+)= P Q^T; hi lo, lo hi, hi hi. P, Q: planes of an operand; q_mn: Q is X as the rows of the reduction
+  auto issue = [&](uint32_t acc_col, uint32_t p0, int p_plane, uint32_t q0, int q_plane, bool q_mn, int k_steps, int n, bool add) {
+    if (warp == 0 && elect_one()) {
+      const uint32_t idesc = make_instr_desc(0, 0, 0, q_mn ? 1 : 0, 128, (uint32_t)n);
+      uint32_t on = add ? 1u : 0u;
+      for (int seg = SPLIT ? 0 : 2; seg < 3; ++seg) {
+        const uint32_t pb = p0 + (seg == 1 ? p_plane : 0), qb = q0 + (seg == 0 ? q_plane : 0);
+        for (int s = 0; s < k_steps; ++s) {
+          const uint32_t k_off = (s >> 2) * SM_PANEL + (s & 3) * 32;          // K-major: 16 columns further
+          const uint64_t dp = make_smem_desc(pb + k_off, 16, 1024);
+          const uint64_t dq = q_mn ? make_smem_desc(qb + s * (16 * 128), SM_PANEL, 1024) : make_smem_desc(qb + k_off, 16, 1024);
+          mma_bf16(tmem_slot + acc_col, dp, dq, idesc, on);
+          on = 1u;
+        }
+      }
+      mma_commit(mma_bar);
+    }
+    __syncwarp();
+  };
+
+  // ---- X scaled: operands, and a X for the products to add to
+  for (int c0 = part4 * 32; c0 < slice; c0 += 128) {
+    uint32_t w[32];
+    float v[32];
+    tmem_ld_32x32(tmem_row + S::X_COL + c0, w);
+    tmem_ld_wait();
+#pragma unroll
+    for (int i = 0; i < 32; ++i) {
+      v[i] = fine ? __uint_as_float(w[i]) * finv : (float)((double)__uint_as_float(w[i]) * inv);
+      w[i] = __float_as_uint(SPLIT ? v[i] : v[i] * (g.a * NS_SCALE));
+    }
+    sm_put_operand<SPLIT>(xs, S::X_BYTES, row, c0, v);
+    tmem_st_32x32(tmem_row + S::X_COL + c0, w);
+  }
+  tmem_st_wait();
+
+  for (int step = 0; step < g.steps; ++step) {
+    // A = X X^T
+    publish(false);
+    issue(S::ACC_COL, xs_addr, S::X_BYTES, xs_addr, S::X_BYTES, false, slice >> 4, 128, false);
+    mma_wait();
+    if (ctas == 1) {
+      uint32_t w[32];
+      float v[32];
+      tmem_ld_32x32(tmem_row + S::ACC_COL + part4 * 32, w);
+      tmem_ld_wait();
+#pragma unroll
+      for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(w[i]) * NS_UNSCALE;
+      sm_put_operand<SPLIT>(as, S::F_BYTES, row, part4 * 32, v);
+      publish(false);
+    } else {
+      // this CTA's share as 512-byte rows of 16-byte pieces, XOR-ed with the row
+      uint32_t w[32];
+      tmem_ld_32x32(tmem_row + S::ACC_COL + part4 * 32, w);
+      tmem_ld_wait();
+#pragma unroll
+      for (int q = 0; q < 8; ++q)
+        *reinterpret_cast<uint4*>(part + row * 512 + (((part4 * 8 + q) ^ (row & 7)) << 4)) = make_uint4(w[4 * q], w[4 * q + 1], w[4 * q + 2], w[4 * q + 3]);
+      tc_fence_before_sync();
+      cluster_sync_all();
+      // rows rank * 128 / ctas ...: sum over the CTAs, result to all of them
+      const int rows_here = 128 / (int)ctas;
+      for (int t = tid; t < rows_here * 32; t += SM_THREADS) {
+        const int r = (int)rank * rows_here + (t >> 5), q = t & 31;
+        const uint32_t at = smem_u32(part + r * 512 + ((q ^ (r & 7)) << 4));
+        float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        for (uint32_t c0 = 0; c0 < ctas; c0 += 8) {
+          float4 v[8];
+#pragma unroll
+          for (uint32_t c = 0; c < 8; ++c)
+            if (c0 + c < ctas) v[c] = ld_dsmem_f4(at, c0 + c);
+#pragma unroll
+          for (uint32_t c = 0; c < 8; ++c)
+            if (c0 + c < ctas) { sum.x += v[c].x; sum.y += v[c].y; sum.z += v[c].z; sum.w += v[c].w; }
+        }
+        sum.x *= NS_UNSCALE; sum.y *= NS_UNSCALE; sum.z *= NS_UNSCALE; sum.w *= NS_UNSCALE;
+        const uint2 hi = make_uint2(pack_half2(sum.x, sum.y), pack_half2(sum.z, sum.w));
+        const float2 h0 = unpack_half2(hi.x), h1 = unpack_half2(hi.y);
+        const uint2 lo = make_uint2(pack_half2(sum.x - h0.x, sum.y - h0.y), pack_half2(sum.z - h1.x, sum.w - h1.y));
+        const int col = q * 4;
+        const uint32_t to = smem_u32(as + (col >> 6) * SM_PANEL + sm_piece(r, (col & 63) >> 3) + (col & 7) * 2);
+        for (uint32_t c = 0; c < ctas; ++c) {
+          st_dsmem_u2(to, c, hi);
+          if (SPLIT) st_dsmem_u2(to + S::F_BYTES, c, lo);
+        }
+      }
+      publish(true);
+    }
+    // B = b A + c A A
+    issue(S::ACC_COL, as_addr, S::F_BYTES, as_addr, S::F_BYTES, false, 8, 128, false);
+    mma_wait();
+    {
+      const int c0 = part4 * 32;
+      uint32_t w[32];
+      float v[32];
+      tmem_ld_32x32(tmem_row + S::ACC_COL + c0, w);
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const uint8_t* at = as + (c0 >> 6) * SM_PANEL + sm_piece(row, ((c0 & 63) >> 3) + q);
+        const uint4 hi = *reinterpret_cast<const uint4*>(at);
+        const uint32_t hw[4] = {hi.x, hi.y, hi.z, hi.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float2 f = unpack_half2(hw[i]);
+          v[8 * q + 2 * i] = f.x; v[8 * q + 2 * i + 1] = f.y;
+        }
+        if (SPLIT) {
+          const uint4 lo = *reinterpret_cast<const uint4*>(at + S::F_BYTES);
+          const uint32_t lw[4] = {lo.x, lo.y, lo.z, lo.w};
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float2 f = unpack_half2(lw[i]);
+            v[8 * q + 2 * i] += f.x; v[8 * q + 2 * i + 1] += f.y;
+          }
+        }
+      }
+      tmem_ld_wait();
+#pragma unroll
+      for (int i = 0; i < 32; ++i) v[i] = fmaf(g.b, v[i], (g.c * NS_UNSCALE) * __uint_as_float(w[i]));
+      sm_put_operand<SPLIT>(bs, S::F_BYTES, row, c0, v);
+    }
+    publish(false);
+    // X <- a X + B X
+    issue(S::BX_COL, bs_addr, S::F_BYTES, xs_addr, S::X_BYTES, true, 8, slice, !SPLIT);
+    mma_wait();
+    if (!SPLIT && step + 1 == g.steps) break;
+#pragma unroll 1
+    for (int c0 = part4 * 32; c0 < slice; c0 += 128) {
+      uint32_t w[32];
+      float v[32];
+      tmem_ld_32x32(tmem_row + S::X_COL + c0, w);
+      if constexpr (SPLIT) {
+        uint32_t bx[32];
+        tmem_ld_32x32(tmem_row + S::BX_COL + c0, bx);
+        tmem_ld_wait();
+#pragma unroll
+        for (int i = 0; i < 32; ++i) {
+          v[i] = fmaf(g.a, __uint_as_float(w[i]), __uint_as_float(bx[i]) * NS_UNSCALE);
+          w[i] = __float_as_uint(v[i]);
+        }
+      } else {
+        tmem_ld_wait();
+#pragma unroll
+        for (int i = 0; i < 32; ++i) {
+          v[i] = __uint_as_float(w[i]) * NS_UNSCALE;
+          w[i] = __float_as_uint(__uint_as_float(w[i]) * g.a);
+        }
+      }
+      sm_put_operand<SPLIT>(xs, S::X_BYTES, row, c0, v);
+      tmem_st_32x32(tmem_row + S::X_COL + c0, w);
+    }
+    tmem_st_wait();
+  }
+
+  // ---- the result, or the parameter update
+  void* out = e.out[z];
+  for (int p = 0; p < panels; ++p) {
+    if (part4 < 2) {
+      uint32_t w[32];
+      tmem_ld_32x32(tmem_row + S::X_COL + p * 64 + part4 * 32, w);
+      tmem_ld_wait();
+#pragma unroll
+      for (int c = 0; c < 32; ++c) staging[row * SM_STAGE_LD + part4 * 32 + c] = __uint_as_float(w[c]) * (SPLIT ? NS_UNSCALE : NS_UNSCALE * NS_UNSCALE);
+    }
+    __syncthreads();
+#pragma unroll 1
+    for (int n0 = 0; n0 < ACCESSES; n0 += AT_ONCE) {
+      VecF<V> v[AT_ONCE];
+#pragma unroll
+      for (int q = 0; q < AT_ONCE; ++q) {
+        int i, j;
+        if (!coord(p, n0 + q, i, j) || !e.momentum) continue;
+        v[q] = load_vec<V>(out, e.out_dtype, g.tall ? (int64_t)(s0 + j) * e.cols + i : (int64_t)i * e.cols + s0 + j);
+      }
+#pragma unroll
+      for (int q = 0; q < AT_ONCE; ++q) {
+        int i, j;
+        if (!coord(p, n0 + q, i, j)) continue;
+#pragma unroll
+        for (int x = 0; x < V; ++x) {
+          const float o = staging[(i + (g.tall ? x : 0)) * SM_STAGE_LD + (j & 63) + (g.tall ? 0 : x)];
+          v[q].e[x] = e.momentum ? fmaf(-e.step, o, v[q].e[x] * e.decay) : o;
+        }
+        store_vec<V>(out, e.out_dtype, g.tall ? (int64_t)(s0 + j) * e.cols + i : (int64_t)i * e.cols + s0 + j, v[q]);
+      }
+    }
+    __syncthreads();
+  }
+
+  tc_fence_before_sync();
+  __syncthreads();
+  if (warp == 0) {
+    tc_fence_after_sync();
+    tmem_dealloc(tmem_slot, S::TMEM_COLS);
+  }
+  if (ctas > 1) cluster_sync_all();
+}
+
+// ---------------------------------------------------------------------------------------
 // host side
 // ---------------------------------------------------------------------------------------
 typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
@@ -944,7 +1388,6 @@ static NsSpace ns_space(int64_t batch, int64_t rows, int64_t cols) {
   return w;
 }
 
-int64_t ns_workspace_bytes(int64_t batch, int64_t rows, int64_t cols) { return ns_space(batch, rows, cols).total; }
 
 template <int V>
 static void ns_begin(const NsEnds& e, int norm_blocks, int blocks, cudaStream_t st) {
@@ -952,10 +1395,72 @@ static void ns_begin(const NsEnds& e, int norm_blocks, int blocks, cudaStream_t 
   ns_scale_kernel<V><<<dim3(blocks, e.batch), ENDS_THREADS, 0, st>>>(e, norm_blocks);
 }
 
+// Whether four elements an access fit every row of every matrix.
+static bool ns_vec4(const NsEnds& e) {
+  const int in_size = e.grad_dtype == ELEM_F32 ? 4 : 2, out_size = e.out_dtype == ELEM_F32 ? 4 : 2;
+  bool vec = e.cols % 4 == 0 && e.grad_ld % 4 == 0;
+  for (int z = 0; z < e.batch && vec; ++z) {
+    vec = reinterpret_cast<uintptr_t>(e.grad[z]) % (4 * in_size) == 0 && reinterpret_cast<uintptr_t>(e.out[z]) % (4 * out_size) == 0 &&
+          reinterpret_cast<uintptr_t>(e.info[z]) % (4 * in_size) == 0 && reinterpret_cast<uintptr_t>(e.moment[z]) % 16 == 0;
+  }
+  return vec;
+}
+
+template <bool SPLIT, int V>
+static const char* launch_small(const NsCall& call, int sms, Status* status, cudaStream_t st) {
+  using S = SmShape<SPLIT>;
+  NsSmall g;
+  g.tall = call.ends.rows > call.ends.cols;
+  g.k = g.tall ? call.ends.cols : call.ends.rows;
+  g.wide = g.tall ? call.ends.rows : call.ends.cols;
+  g.steps = call.steps;
+  g.a = call.c[0];
+  g.b = call.c[1];
+  g.c = call.c[2];
+  g.ctas = 1;
+  // As few CTAs as hold the matrix: one 128 x 512 matrix takes 50 us on 2 CTAs and 43 us on 8, 48 of them 51 and 168 us.
+  while (g.ctas * S::SLICE < g.wide) g.ctas *= 2;
+  g.slice = ((g.wide + g.ctas - 1) / g.ctas + 63) / 64 * 64;
+  auto kernel = ns_small_kernel<SPLIT, V>;
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM) != cudaSuccess) return "orthogonalize: shared memory";
+  if (g.ctas > 8 && cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess)
+    return "orthogonalize: cluster size";
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(call.ends.batch * g.ctas));
+  cfg.blockDim = dim3(SM_THREADS);
+  cfg.dynamicSmemBytes = S::SMEM;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = (unsigned)g.ctas;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, call.ends, g, status) == cudaSuccess ? nullptr : "ns_small launch failed";
+}
+
+// A side of at most 128 and a long side of at most 2048: 8 CTAs with slices of 256 columns, 16 with slices of 128.
+static bool ns_is_small(int64_t rows, int64_t cols, int steps, int pairs) {
+  const int64_t k = rows < cols ? rows : cols, wide = rows < cols ? cols : rows;
+  return steps > 0 && k <= 128 && wide <= (pairs ? 16 * SmShape<true>::SLICE : 8 * SmShape<false>::SLICE);
+}
+
+int64_t ns_workspace_bytes(int64_t batch, int64_t rows, int64_t cols, int steps, int pairs) {
+  return ns_is_small(rows, cols, steps, pairs) ? 0 : ns_space(batch, rows, cols).total;
+}
+
 const char* launch_orthogonalize(const NsCall& call, Status* status, cudaStream_t st) {
   const int64_t batch = call.ends.batch, rows = call.ends.rows, cols = call.ends.cols;
   if (batch < 1 || batch > NS_MAX_BATCH || rows < 1 || cols < 1) return "orthogonalize: sizes";
   if (rows > (1 << 20) || cols > (1 << 20)) return "orthogonalize: matrix too large";
+  int dev = 0, sms = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
+    return "orthogonalize: device";
+  const bool vec = ns_vec4(call.ends);
+  if (ns_is_small(rows, cols, call.steps, call.pairs)) {
+    if (call.pairs) return vec ? launch_small<true, 4>(call, sms, status, st) : launch_small<true, 1>(call, sms, status, st);
+    return vec ? launch_small<false, 4>(call, sms, status, st) : launch_small<false, 1>(call, sms, status, st);
+  }
   const NsSpace w = ns_space(batch, rows, cols);
   __half* base = reinterpret_cast<__half*>(call.workspace);
   __half* x[2] = {base, base + w.x};                       // each: hi planes of the batch, then lo planes
@@ -964,10 +1469,6 @@ const char* launch_orthogonalize(const NsCall& call, Status* status, cudaStream_
   const int64_t lo_x = w.x / 2, lo_k = w.k / 2;
   uint8_t* tail = reinterpret_cast<uint8_t*>(call.workspace) + 2 * w.partial;
   const bool tall = rows > cols;
-
-  int dev = 0, sms = 0;
-  if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
-    return "orthogonalize: device";
 
   NsPlan g;
   memset(&g, 0, sizeof(g));
@@ -980,13 +1481,6 @@ const char* launch_orthogonalize(const NsCall& call, Status* status, cudaStream_
   e.partial = reinterpret_cast<double*>(tail);
   e.done = reinterpret_cast<uint32_t*>(tail + batch * NS_NORM_BLOCKS * sizeof(double));
   e.next_item = e.done + batch;
-  // four elements an access where every row of every matrix allows it
-  const int in_size = e.grad_dtype == ELEM_F32 ? 4 : 2, out_size = e.out_dtype == ELEM_F32 ? 4 : 2;
-  bool vec = cols % 4 == 0 && e.grad_ld % 4 == 0;
-  for (int64_t z = 0; z < batch && vec; ++z) {
-    vec = reinterpret_cast<uintptr_t>(e.grad[z]) % (4 * in_size) == 0 && reinterpret_cast<uintptr_t>(e.out[z]) % (4 * out_size) == 0 &&
-          reinterpret_cast<uintptr_t>(e.info[z]) % (4 * in_size) == 0 && reinterpret_cast<uintptr_t>(e.moment[z]) % 16 == 0;
-  }
   const int64_t per_row = (cols + (vec ? 3 : 0)) / (vec ? 4 : 1);
   e.tpr_log2 = 0;
   while (e.tpr_log2 < 8 && (1 << e.tpr_log2) < per_row) ++e.tpr_log2;

@@ -49,6 +49,13 @@ struct NsPlan {
   uint32_t* next_item;
 };
 
+// A call whose matrices have a side of at most 128 (see ns_small_kernel).
+struct NsSmall {
+  int k, wide, tall, steps;
+  int ctas, slice;                     // CTAs per matrix, columns of X per CTA
+  float a, b, c;
+};
+
 struct NsCall {
   NsEnds ends;
   void* workspace;                     // ns_workspace_bytes(), 256-byte aligned
@@ -56,7 +63,7 @@ struct NsCall {
   float c[3];                          // coefficients a, b, c of the step
 };
 
-int64_t ns_workspace_bytes(int64_t batch, int64_t rows, int64_t cols);
+int64_t ns_workspace_bytes(int64_t batch, int64_t rows, int64_t cols, int steps, int pairs);
 const char* launch_orthogonalize(const NsCall& call, Status* status, cudaStream_t st);
 
 }  // namespace gd

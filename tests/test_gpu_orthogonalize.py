@@ -236,3 +236,19 @@ def test_engine_gradient_of_the_table_is_the_sum_by_token():
     cu.linear_cross_entropy(leaf.reshape(-1, 64), w, tok.reshape(-1), 512, False).backward()
     assert w.main_grad.any() and leaf.grad.any()
     assert torch.equal(both, ops.embedding_grad(tok, leaf.grad, 512, 2.0, out=w.main_grad))
+
+
+# sides around 128: one cluster keeps the matrix, with 1 to 16 CTAs; long sides at and around the slices they hold
+@pytest.mark.parametrize("n,r,c", [(2, 128, 256), (1, 127, 257), (3, 100, 64), (2, 128, 512), (2, 513, 90), (1, 20, 1000), (1, 128, 1025),
+                                   (2, 1024, 128), (1, 33, 2048), (1, 2049, 128), (1, 128, 2048), (40, 17, 300)])
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_small_side(n, r, c, dtype):
+    g = torch.Generator().manual_seed(r * 1000 + c)
+    x = gradient_like(g, n, r, c, DEV).to(dtype)
+    got = ops.orthogonalize(x)
+    want, tol = orthogonalize_bound(x.cpu(), dtype)
+    for i in range(n):
+        assert rel(got[i], want[i]) <= 2 * tol, (i, rel(got[i], want[i]), tol)
+    assert torch.equal(got, ops.orthogonalize(x))
+    if n > 1:       # the others' number does not change a matrix
+        assert torch.equal(got[-1], ops.orthogonalize(x[-1]))
