@@ -1085,14 +1085,15 @@ void check_tokens(const Tensor& tokens, const Tensor& like) {
   TORCH_CHECK(tokens.is_contiguous(), "tokens must be contiguous");
 }
 
-void token_lookup(const Tensor& tokens, const Tensor& table, double scale, Tensor out) {
+Tensor token_lookup(const Tensor& tokens, const Tensor& table, double scale) {
   c10::cuda::CUDAGuard guard(table.device());
   OpRange gd_range_(__func__);
   check_cuda(table, "table");
-  check_cuda(out, "out");
   check_tokens(tokens, table);
-  TORCH_CHECK(table.dim() == 2 && out.is_contiguous() && out.scalar_type() == table.scalar_type() &&
-              out.device() == table.device() && out.numel() == tokens.numel() * table.size(1), "token_lookup: out must be (tokens, width) of the table's type");
+  TORCH_CHECK(table.dim() == 2, "token_lookup: the table is a matrix");
+  std::vector<int64_t> shape(tokens.sizes().begin(), tokens.sizes().end());
+  shape.push_back(table.size(1));
+  Tensor out = at::empty(shape, table.options());
   gd::TokenLookupArgs a{};
   a.tokens = tokens.data_ptr();
   a.wide = tokens.scalar_type() == at::kLong;
@@ -1105,37 +1106,44 @@ void token_lookup(const Tensor& tokens, const Tensor& table, double scale, Tenso
   a.scale = (float)scale;
   a.out = out.data_ptr();
   GD_LAUNCH(gd::launch_token_lookup(a, status_ptr(table), stream_of(table)));
+  return out;
 }
 
-void token_grad(const Tensor& tokens, const Tensor& grad, double scale, bool add, Tensor out) {
+// out given: fp32, added to. Otherwise a dense gradient of num_rows rows in grad's type.
+Tensor token_grad(const Tensor& tokens, const Tensor& grad, double scale, int64_t num_rows, OptT out) {
   c10::cuda::CUDAGuard guard(grad.device());
   OpRange gd_range_(__func__);
   check_cuda(grad, "grad");
-  check_cuda(out, "out");
   check_tokens(tokens, grad);
-  TORCH_CHECK(grad.dim() == 2 && out.dim() == 2 && out.is_contiguous() && out.device() == grad.device() &&
-              grad.size(0) == tokens.numel() && out.size(1) == grad.size(1), "token_grad: grad is (tokens, width), out (vocab, width)");
-  TORCH_CHECK(out.scalar_type() == (add ? at::kFloat : grad.scalar_type()), "token_grad: out has the wrong type");
-  if (!add) out.zero_();
-  const auto words = at::TensorOptions().device(grad.device());
-  const int64_t n = tokens.numel();
-  Tensor sort = at::empty({4 * n}, words.dtype(at::kInt));
-  Tensor partial = at::empty({gd::token_grad_partial_floats(n, grad.size(1))}, words.dtype(at::kFloat));
+  TORCH_CHECK(grad.dim() == 2 && grad.size(0) == tokens.numel() && num_rows >= 0, "token_grad: grad is (tokens, width)");
+  const bool add = out.has_value();
+  if (add) {
+    check_cuda(*out, "out");
+    TORCH_CHECK(out->dim() == 2 && out->is_contiguous() && out->device() == grad.device() && out->scalar_type() == at::kFloat &&
+                out->size(0) == num_rows && out->size(1) == grad.size(1), "token_grad: out is (num_rows, width) in float32");
+  }
+  Tensor to = add ? *out : at::empty({num_rows, grad.size(1)}, grad.options());
+  const int64_t n = tokens.numel(), words = gd::token_grad_sort_words(n), partial = gd::token_grad_partial_floats(n, grad.size(1));
+  Tensor space;
   gd::TokenGradArgs a{};
+  if (words + partial > 0) {
+    space = at::empty({(words + 3) / 4 * 4 + partial}, grad.options().dtype(at::kInt));
+    a.sort = reinterpret_cast<uint32_t*>(space.data_ptr());
+    a.partial = reinterpret_cast<float*>(space.data_ptr()) + (words + 3) / 4 * 4;
+  }
   a.tokens = tokens.data_ptr();
   a.wide = tokens.scalar_type() == at::kLong;
   a.n = n;
   a.grad = grad.data_ptr();
-  a.vocab = out.size(0);
+  a.vocab = num_rows;
   a.width = grad.size(1);
   a.grad_ld = grad.stride(0);
   a.dtype = elem_type(grad, "grad");
   a.scale = (float)scale;
   a.add = add;
-  a.out = out.data_ptr();
-  a.sort = reinterpret_cast<uint32_t*>(sort.data_ptr());
-  a.partial = partial.data_ptr<float>();
+  a.out = to.data_ptr();
   GD_LAUNCH(gd::launch_token_grad(a, status_ptr(grad), stream_of(grad)));
+  return to;
 }
 
 // ---- Newton-Schulz ------------------------------------------------------------------------------
@@ -1265,8 +1273,8 @@ TORCH_LIBRARY(gdnet_b200, m) {
   m.def("cross_entropy(Tensor(a!) logits, Tensor targets, Tensor(b!) row_loss, Tensor inv_count, int vocab, int ignore_index, float grad_scale, bool write_grad) -> ()", &cross_entropy);
   m.def("mem_read_fwd(Tensor q, Tensor gamma, Tensor e, Tensor tags, Tensor vals, Tensor alpha, Tensor(a!) w, Tensor(b!) out) -> ()", &mem_read_fwd);
   m.def("mem_read_bwd(Tensor d_out, Tensor q, Tensor gamma, Tensor e, Tensor tags, Tensor vals, Tensor w, Tensor alpha, Tensor(a!) d_q, Tensor(b!) d_gamma, Tensor(c!) d_e, Tensor(d!) d_tags, Tensor(e!) d_vals, Tensor(f!) d_alpha) -> ()", &mem_read_bwd);
-  m.def("token_lookup(Tensor tokens, Tensor table, float scale, Tensor(a!) out) -> ()", &token_lookup);
-  m.def("token_grad(Tensor tokens, Tensor grad, float scale, bool add, Tensor(a!) out) -> ()", &token_grad);
+  m.def("token_lookup(Tensor tokens, Tensor table, float scale) -> Tensor", &token_lookup);
+  m.def("token_grad(Tensor tokens, Tensor grad, float scale, int num_rows, Tensor(a!)? out) -> Tensor", &token_grad);
   m.def("orthogonalize(Tensor x, Tensor(a!) out, int steps, float[] c, float eps, bool pairs) -> ()", &orthogonalize);
   m.def("muon_update(Tensor(a!)[] params, Tensor[] grads, Tensor[] infos, Tensor(b!)[] moments, Tensor? scalars, float beta, float mu, bool nesterov, float decay, float step, int steps, float[] c, float eps, bool pairs) -> ()", &muon_update);
   m.def("grad_dots(Tensor gt, Tensor? gi, Tensor(a!) sums) -> ()", &grad_dots);

@@ -327,13 +327,14 @@ struct TokenGradArgs {
   int64_t vocab, width, grad_ld;
   int dtype;            // ElemType of grad
   float scale;
-  int add;              // 1: out is fp32 and is added to; 0: out has grad's type, rows of absent ids are left as they are
+  int add;              // 1: out is fp32 and is added to; 0: out has grad's type, rows of absent ids become zero
   void* out;            // (vocab, width) contiguous
-  uint32_t* sort;       // 4 n words
+  uint32_t* sort;       // token_grad_sort_words(), 8-byte aligned
   float* partial;       // token_grad_partial_floats()
 };
 
 const char* launch_token_lookup(const TokenLookupArgs& a, Status* status, cudaStream_t st);
+int64_t token_grad_sort_words(int64_t n);
 int64_t token_grad_partial_floats(int64_t n, int64_t width);
 const char* launch_token_grad(const TokenGradArgs& a, Status* status, cudaStream_t st);
 

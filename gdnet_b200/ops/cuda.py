@@ -34,18 +34,15 @@ class _CountingOps:
     def __init__(self, ns):
         self._ns = ns
         self.launches = 0
-        self._cache = {}
 
-    def __getattr__(self, name):
-        fn = self._cache.get(name)
-        if fn is None:
-            op = getattr(self._ns, name)
+    def __getattr__(self, name):          # the first use of an op; later ones find the attribute
+        op = getattr(self._ns, name).default
 
-            def fn(*args, _op=op, **kw):
-                self.launches += 1
-                return _op(*args, **kw)
+        def fn(*args, _op=op, **kw):
+            self.launches += 1
+            return _op(*args, **kw)
 
-            self._cache[name] = fn
+        setattr(self, name, fn)
         return fn
 
 
@@ -794,9 +791,7 @@ class _EmbeddingFn(torch.autograd.Function):
 
 
 def _embedding_fwd(tokens, weight, scale):
-    out = torch.empty(*tokens.shape, weight.shape[1], dtype=weight.dtype, device=weight.device)
-    K.token_lookup(tokens.contiguous(), weight.detach(), scale, out)
-    return out
+    return K.token_lookup(tokens if tokens.is_contiguous() else tokens.contiguous(), weight, scale)
 
 
 def embedding(tokens, weight, scale: float = 1.0):
@@ -808,16 +803,13 @@ def embedding(tokens, weight, scale: float = 1.0):
 
 def embedding_grad(tokens, grad, num_rows: int, scale: float = 1.0, out=None):
     """Sums of the rows of ``grad`` over equal tokens: dense in ``grad``'s type, or added into the fp32 ``out``."""
-    width = grad.shape[-1]
-    g = grad.detach().reshape(tokens.numel(), width)
-    if g.stride(-1) != 1 and width != 1:
+    g = grad if grad.dim() == 2 else grad.reshape(tokens.numel(), grad.shape[-1])
+    if g.stride(-1) != 1 and g.shape[-1] != 1:
         g = g.contiguous()
-    add = out is not None
-    if not add:
-        out = torch.empty(num_rows, width, dtype=grad.dtype, device=grad.device)
-    K.token_grad(tokens.contiguous(), g, scale, add, out)
-    if add:
-        torch.autograd.graph.increment_version(out)
+    if out is None:
+        return K.token_grad(tokens if tokens.is_contiguous() else tokens.contiguous(), g, scale, num_rows, None)
+    K.token_grad(tokens if tokens.is_contiguous() else tokens.contiguous(), g, scale, num_rows, out)
+    torch.autograd.graph.increment_version(out)
     return out
 
 
