@@ -496,6 +496,17 @@ __device__ __forceinline__ void ns_chain_body(const NsPlan& g, Status* status) {
       }
       __syncwarp();
     };
+    // This warp's part of a tile of matrix z is written: count it. `behind`: stores of a later tile may still be on their way.
+    int uncounted = -1;
+    auto count_tile = [&](int z, bool behind) {
+      if (elect_one()) {
+        if (behind) bulk_wait_but_one();
+        else bulk_wait_all();
+        fence_proxy_async_global();
+        asm volatile("red.release.gpu.global.add.u32 [%0], 1;" ::"l"(g.done + z) : "memory");
+      }
+      __syncwarp();
+    };
     auto aux_begin = [&]() {
       if (t.phase == 0) return;
       fence_proxy_async_global();      // the item was handed out after what it reads was written
@@ -591,6 +602,10 @@ __device__ __forceinline__ void ns_chain_body(const NsPlan& g, Status* status) {
           bulk_commit_group();
         }
         __syncwarp();
+        if (uncounted >= 0) {
+          count_tile(uncounted, true);
+          uncounted = -1;
+        }
       };
 
       if constexpr (SPLIT) {
@@ -644,23 +659,21 @@ __device__ __forceinline__ void ns_chain_body(const NsPlan& g, Status* status) {
         }
       }
       if (!ok) break;
-      // The next item's linear term can be asked for before this one's stores are complete, but not waited for: what
-      // it reads may depend on the count below.
+      // The next item's linear term can be asked for before this one's stores are complete, but an item that is not handed out
+      // yet cannot be waited for: what it reads may depend on the count below. If the next item is there and its
+      // accumulator too, this tile is counted after the next one's first chunk, when its stores have long completed.
       const int z_done = t.z;
-      const bool there = ns_item_there(bars, it + 1);
+      bool there = ns_item_there(bars, it + 1), busy = false;
       if (there) {
         t = ns_next_item(bars, it + 1, status);
         if (t.live) {
           corner();
           aux_begin();
+          busy = chunks > 0 && __shfl_sync(0xffffffffu, lane == 0 ? mbar_test_wait(afull0 + 8 * acc, acc_ph) : 0u, 0) != 0;
         }
       }
-      if (elect_one()) {               // this warp's part of the tile is written: count it
-        bulk_wait_all();
-        fence_proxy_async_global();
-        asm volatile("red.release.gpu.global.add.u32 [%0], 1;" ::"l"(g.done + z_done) : "memory");
-      }
-      __syncwarp();
+      if (busy) uncounted = z_done;
+      else count_tile(z_done, false);
       if (!there) {
         t = ns_next_item(bars, it + 1, status);
         if (t.live) {
