@@ -2,6 +2,7 @@
 // Every op validates device, dtype, contiguity of the innermost dimension and alignment on the
 // host, launches on the current CUDA stream and never synchronises.
 #include <ATen/ATen.h>
+#include <ATen/cuda/CUDAEvent.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/library.h>
@@ -10,6 +11,8 @@
 
 #include <algorithm>
 #include <cstdlib>
+#include <mutex>
+#include <optional>
 
 #include "comm.h"
 #include "gemm_sm100.h"
@@ -1165,22 +1168,26 @@ void ns_setup(gd::NsCall& call, int64_t rows, int64_t cols, int64_t steps, at::A
   for (int i = 0; i < 3; ++i) call.c[i] = (float)c[i];
 }
 
-void orthogonalize(const Tensor& x, Tensor out, int64_t steps, at::ArrayRef<double> c, double eps, bool pairs) {
-  c10::cuda::CUDAGuard guard(x.device());
+Tensor orthogonalize(const Tensor& x_in, at::ScalarType out_dtype, int64_t steps, at::ArrayRef<double> c, double eps, bool pairs) {
+  c10::cuda::CUDAGuard guard(x_in.device());
   OpRange gd_range_(__func__);
-  check_cuda(x, "x");
-  check_cuda(out, "out");
-  TORCH_CHECK(x.dim() == 3 && out.sizes() == x.sizes() && out.is_contiguous() && out.device() == x.device(), "orthogonalize: (n, rows, cols) tensors");
-  const int64_t n = x.size(0), rows = x.size(1), cols = x.size(2);
-  if (x.numel() == 0) return;
+  TORCH_CHECK(x_in.is_cuda() && x_in.dim() >= 2, "orthogonalize: CUDA matrices");
+  Tensor out = at::empty(x_in.sizes(), x_in.options().dtype(out_dtype).memory_format(at::MemoryFormat::Contiguous));
+  if (out.numel() == 0) return out;
+  const int64_t rows = x_in.size(-2), cols = x_in.size(-1), n = x_in.numel() / (rows * cols);
+  Tensor x = x_in.dim() == 3 ? x_in : x_in.reshape({n, rows, cols});
+  if (cols > 1 && x.stride(2) != 1) x = x.contiguous();
   gd::NsCall call{};
   ns_setup(call, rows, cols, steps, c, eps, pairs);
   call.ends.grad_dtype = elem_type(x, "x");
   call.ends.out_dtype = elem_type(out, "out");
   call.ends.grad_ld = x.stride(1);
-  const int64_t group = ns_group(n, rows, cols);
-  Tensor space = at::empty({gd::ns_workspace_bytes(group, rows, cols, call.steps, call.pairs)}, x.options().dtype(at::kByte));
-  call.workspace = space.data_ptr();
+  const int64_t group = ns_group(n, rows, cols), space_bytes = gd::ns_workspace_bytes(group, rows, cols, call.steps, call.pairs);
+  Tensor space;
+  if (space_bytes > 0) {
+    space = at::empty({space_bytes}, x.options().dtype(at::kByte));
+    call.workspace = space.data_ptr();
+  }
   for (int64_t i0 = 0; i0 < n; i0 += group) {
     const int64_t count = std::min(group, n - i0);
     call.ends.batch = (int)count;
@@ -1190,56 +1197,135 @@ void orthogonalize(const Tensor& x, Tensor out, int64_t steps, at::ArrayRef<doub
     }
     GD_LAUNCH(gd::launch_orthogonalize(call, status_ptr(x), stream_of(x)));
   }
+  return out;
 }
 
+// The stream that independent groups of one update run on beside the caller's (one per device, made on first use).
+c10::cuda::CUDAStream muon_side_stream(int device) {
+  static std::mutex mutex;
+  static std::vector<std::optional<c10::cuda::CUDAStream>> per_device(64);
+  std::lock_guard<std::mutex> lock(mutex);
+  TORCH_CHECK(device >= 0 && device < 64, "bad device index");
+  if (!per_device[device].has_value()) per_device[device] = c10::cuda::getStreamFromPool(false, (c10::DeviceIndex)device);
+  return *per_device[device];
+}
+
+// params, grads, (infos,) moments: contiguous matrices or banks of matrices (n, rows, cols). Matrices of one shape and type share
+// their launches; groups of different shapes are independent chains of dependent products, so every other group
+// runs on a second stream, which joins the caller's before this returns.
 void muon_update(at::TensorList params, at::TensorList grads, at::TensorList infos, at::TensorList moments, OptT scalars,
-                 double beta, double mu, bool nesterov, double decay, double step, int64_t steps, at::ArrayRef<double> c, double eps,
-                 bool pairs) {
-  const int64_t n = (int64_t)params.size();
+                 double beta, double mu, bool nesterov, double lr, double weight_decay, double update_scale, int64_t steps,
+                 at::ArrayRef<double> c, double eps) {
+  const size_t n = params.size();
+  TORCH_CHECK_VALUE(grads.size() == n && moments.size() == n && (infos.empty() || infos.size() == n),
+                    "muon_update_: params, grads, momenta (and info_grads) must have the same length");
   if (n == 0) return;
-  const Tensor& first = params[0];
-  c10::cuda::CUDAGuard guard(first.device());
+  const auto device = params[0].device();
+  TORCH_CHECK(device.is_cuda(), "muon_update: CUDA tensors");
+  c10::cuda::CUDAGuard guard(device);
   OpRange gd_range_(__func__);
-  TORCH_CHECK((int64_t)grads.size() == n && (int64_t)moments.size() == n && (infos.empty() || (int64_t)infos.size() == n), "muon_update: one entry per matrix");
-  TORCH_CHECK(first.dim() == 2, "muon_update: matrices");
-  for (int64_t i = 0; i < n; ++i) {
-    const Tensor* ts[4] = {&params[i], &grads[i], &moments[i], infos.empty() ? &grads[i] : &infos[i]};
-    for (const Tensor* t : ts)
-      TORCH_CHECK(t->is_cuda() && t->device() == first.device() && t->is_contiguous() && t->sizes() == first.sizes(),
-                  "muon_update: contiguous matrices of one shape on one device");
-    TORCH_CHECK(params[i].scalar_type() == first.scalar_type() && grads[i].scalar_type() == grads[0].scalar_type() &&
-                (infos.empty() || infos[i].scalar_type() == grads[0].scalar_type()) && moments[i].scalar_type() == at::kFloat,
-                "muon_update: params and gradients of one type each, momentum in float32");
-  }
-  const int64_t rows = first.size(0), cols = first.size(1);
-  if (rows == 0 || cols == 0) return;
-  gd::NsCall call{};
-  ns_setup(call, rows, cols, steps, c, eps, pairs);
-  call.ends.momentum = 1;
-  call.ends.nesterov = nesterov;
-  call.ends.grad_dtype = elem_type(grads[0], "grads");
-  call.ends.out_dtype = elem_type(first, "params");
-  call.ends.grad_ld = cols;
-  if (scalars.has_value()) TORCH_CHECK(scalars->numel() >= 2 && scalars->device() == first.device(), "muon_update: scalars");
-  call.ends.scalars = opt_f32(scalars, "scalars");
-  TORCH_CHECK(infos.empty() || call.ends.scalars != nullptr, "muon_update: information gradients need the projection scalars");
-  call.ends.beta = (float)beta;
-  call.ends.mu = (float)mu;
-  call.ends.decay = (float)decay;
-  call.ends.step = (float)step;
-  const int64_t group = ns_group(n, rows, cols);
-  Tensor space = at::empty({gd::ns_workspace_bytes(group, rows, cols, call.steps, call.pairs)}, first.options().dtype(at::kByte));
-  call.workspace = space.data_ptr();
-  for (int64_t i0 = 0; i0 < n; i0 += group) {
-    const int64_t count = std::min(group, n - i0);
-    call.ends.batch = (int)count;
-    for (int64_t i = 0; i < count; ++i) {
-      call.ends.grad[i] = grads[i0 + i].data_ptr();
-      call.ends.info[i] = infos.empty() ? nullptr : infos[i0 + i].data_ptr();
-      call.ends.moment[i] = moments[i0 + i].data_ptr();
-      call.ends.out[i] = params[i0 + i].data_ptr();
+  auto float_type = [](const Tensor& t) {
+    return t.scalar_type() == at::kBFloat16 || t.scalar_type() == at::kHalf || t.scalar_type() == at::kFloat;
+  };
+  struct Span { uintptr_t lo, hi; bool written; };
+  std::vector<Span> spans;
+  spans.reserve(4 * n);
+  struct Group {
+    int64_t rows, cols;
+    at::ScalarType type, grad_type;
+    std::vector<const void*> grad, info;
+    std::vector<void*> moment, out;
+  };
+  std::vector<Group> groups;
+  for (size_t i = 0; i < n; ++i) {
+    const Tensor& p = params[i];
+    TORCH_CHECK_VALUE(p.dim() == 2 || p.dim() == 3, "muon_update_: entry ", i, " needs matrices, got ", p.sizes());
+    const Tensor* all[4] = {&p, &moments[i], &grads[i], infos.empty() ? nullptr : &infos[i]};
+    for (int k = 0; k < 4; ++k) {
+      if (all[k] == nullptr) continue;
+      const Tensor& t = *all[k];
+      TORCH_CHECK_VALUE(t.sizes() == p.sizes(), "muon_update_: entry ", i, " needs matrices of one shape, got ", p.sizes(), " and ", t.sizes());
+      TORCH_CHECK_VALUE(t.device() == device && t.is_contiguous(), "muon_update_: entry ", i, " must be contiguous and on ", device);
+      const uintptr_t lo = reinterpret_cast<uintptr_t>(t.data_ptr());
+      if (t.numel() > 0) spans.push_back({lo, lo + (uintptr_t)t.nbytes(), k < 2});
     }
-    GD_LAUNCH(gd::launch_orthogonalize(call, status_ptr(first), stream_of(first)));
+    TORCH_CHECK_TYPE(float_type(p) && float_type(grads[i]) && moments[i].scalar_type() == at::kFloat &&
+                     (infos.empty() || infos[i].scalar_type() == grads[i].scalar_type()),
+                     "muon_update_: entry ", i, " has types ", p.scalar_type(), ", ", grads[i].scalar_type(), ", ", moments[i].scalar_type());
+    const int64_t rows = p.size(-2), cols = p.size(-1);
+    if (p.numel() == 0) continue;
+    Group* g = nullptr;
+    for (Group& have : groups)
+      if (have.rows == rows && have.cols == cols && have.type == p.scalar_type() && have.grad_type == grads[i].scalar_type()) g = &have;
+    if (g == nullptr) {
+      groups.push_back(Group{rows, cols, p.scalar_type(), grads[i].scalar_type(), {}, {}, {}, {}});
+      g = &groups.back();
+    }
+    const int64_t step = rows * cols, in_size = (int64_t)grads[i].element_size();
+    for (int64_t z = 0; z < p.numel() / step; ++z) {
+      g->grad.push_back(reinterpret_cast<const char*>(grads[i].data_ptr()) + z * step * in_size);
+      g->info.push_back(infos.empty() ? nullptr : reinterpret_cast<const char*>(infos[i].data_ptr()) + z * step * in_size);
+      g->moment.push_back(reinterpret_cast<char*>(moments[i].data_ptr()) + z * step * 4);
+      g->out.push_back(reinterpret_cast<char*>(p.data_ptr()) + z * step * (int64_t)p.element_size());
+    }
+  }
+  std::sort(spans.begin(), spans.end(), [](const Span& a, const Span& b) { return a.lo < b.lo; });
+  uintptr_t end_any = 0, end_written = 0;
+  for (const Span& s : spans) {
+    TORCH_CHECK_VALUE(s.lo >= (s.written ? end_any : end_written), "muon_update_: entries share memory");
+    end_any = std::max(end_any, s.hi);
+    if (s.written) end_written = std::max(end_written, s.hi);
+  }
+  if (scalars.has_value()) TORCH_CHECK(scalars->numel() >= 2 && scalars->device() == device, "muon_update: scalars");
+  TORCH_CHECK(infos.empty() || scalars.has_value(), "muon_update: information gradients need the projection scalars");
+
+  const auto here = c10::cuda::getCurrentCUDAStream(device.index());
+  const auto side = groups.size() > 1 ? muon_side_stream(device.index()) : here;
+  if (groups.size() > 1) {
+    at::cuda::CUDAEvent begun;
+    begun.record(here);
+    begun.block(side);
+  }
+  for (size_t k = 0; k < groups.size(); ++k) {
+    const Group& g = groups[k];
+    c10::cuda::CUDAStreamGuard on(k % 2 != 0 ? side : here);
+    gd::NsCall call{};
+    ns_setup(call, g.rows, g.cols, steps, c, eps, g.type != at::kBFloat16);
+    call.ends.momentum = 1;
+    call.ends.nesterov = nesterov;
+    call.ends.grad_dtype = g.grad_type == at::kFloat ? gd::ELEM_F32 : (g.grad_type == at::kHalf ? gd::ELEM_F16 : gd::ELEM_BF16);
+    call.ends.out_dtype = g.type == at::kFloat ? gd::ELEM_F32 : (g.type == at::kHalf ? gd::ELEM_F16 : gd::ELEM_BF16);
+    call.ends.grad_ld = g.cols;
+    call.ends.scalars = opt_f32(scalars, "scalars");
+    call.ends.beta = (float)beta;
+    call.ends.mu = (float)mu;
+    call.ends.decay = (float)(1.0 - lr * weight_decay);
+    call.ends.step = (float)(lr * (update_scale >= 0.0 ? update_scale : 0.2 * std::sqrt((double)std::max(g.rows, g.cols))));
+    const int64_t total = (int64_t)g.out.size(), group = ns_group(total, g.rows, g.cols);
+    const int64_t space_bytes = gd::ns_workspace_bytes(group, g.rows, g.cols, call.steps, call.pairs);
+    Tensor space;
+    if (space_bytes > 0) {
+      space = at::empty({space_bytes}, params[0].options().dtype(at::kByte));
+      call.workspace = space.data_ptr();
+    }
+    for (int64_t i0 = 0; i0 < total; i0 += group) {
+      const int64_t count = std::min(group, total - i0);
+      call.ends.batch = (int)count;
+      std::copy_n(g.grad.begin() + i0, count, call.ends.grad);
+      std::copy_n(g.info.begin() + i0, count, call.ends.info);
+      std::copy_n(g.moment.begin() + i0, count, call.ends.moment);
+      std::copy_n(g.out.begin() + i0, count, call.ends.out);
+      GD_LAUNCH(gd::launch_orthogonalize(call, status_ptr(params[0]), (k % 2 != 0 ? side : here).stream()));
+    }
+  }
+  if (groups.size() > 1) {
+    at::cuda::CUDAEvent done;
+    done.record(side);
+    done.block(here);
+  }
+  for (size_t i = 0; i < n; ++i) {
+    if (!params[i].is_inference()) params[i].unsafeGetTensorImpl()->bump_version();
+    if (!moments[i].is_inference()) moments[i].unsafeGetTensorImpl()->bump_version();
   }
 }
 
@@ -1275,8 +1361,8 @@ TORCH_LIBRARY(gdnet_b200, m) {
   m.def("mem_read_bwd(Tensor d_out, Tensor q, Tensor gamma, Tensor e, Tensor tags, Tensor vals, Tensor w, Tensor alpha, Tensor(a!) d_q, Tensor(b!) d_gamma, Tensor(c!) d_e, Tensor(d!) d_tags, Tensor(e!) d_vals, Tensor(f!) d_alpha) -> ()", &mem_read_bwd);
   m.def("token_lookup(Tensor tokens, Tensor table, float scale) -> Tensor", &token_lookup);
   m.def("token_grad(Tensor tokens, Tensor grad, float scale, int num_rows, Tensor(a!)? out) -> Tensor", &token_grad);
-  m.def("orthogonalize(Tensor x, Tensor(a!) out, int steps, float[] c, float eps, bool pairs) -> ()", &orthogonalize);
-  m.def("muon_update(Tensor(a!)[] params, Tensor[] grads, Tensor[] infos, Tensor(b!)[] moments, Tensor? scalars, float beta, float mu, bool nesterov, float decay, float step, int steps, float[] c, float eps, bool pairs) -> ()", &muon_update);
+  m.def("orthogonalize(Tensor x, ScalarType out_dtype, int steps, float[] c, float eps, bool pairs) -> Tensor", &orthogonalize);
+  m.def("muon_update(Tensor(a!)[] params, Tensor[] grads, Tensor[] infos, Tensor(b!)[] moments, Tensor? scalars, float beta, float mu, bool nesterov, float lr, float weight_decay, float update_scale, int steps, float[] c, float eps) -> ()", &muon_update);
   m.def("grad_dots(Tensor gt, Tensor? gi, Tensor(a!) sums) -> ()", &grad_dots);
   m.def("projected_adamw(Tensor(a!) p, Tensor gt, Tensor? gi, Tensor(b!) m, Tensor(c!) v, Tensor scalars, float beta_proj, float lr, float beta1, float beta2, float eps, float weight_decay, int step) -> ()", &projected_adamw);
   m.def("batched_outer_add(Tensor dsts, Tensor ys, Tensor vecs, Tensor coef, Tensor rows, Tensor cols, int max_rows) -> ()", &batched_outer_add);

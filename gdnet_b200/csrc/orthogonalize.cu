@@ -736,7 +736,7 @@ constexpr int ENDS_THREADS = 256;
 constexpr int ENDS_ROWS = 4;
 
 template <int V>
-struct alignas(V * 4) VecF { float e[V]; };
+struct alignas(V < 4 ? V * 4 : 16) VecF { float e[V]; };
 template <int V>
 struct alignas(V * 2) VecH { uint16_t e[V]; };
 
@@ -931,9 +931,10 @@ ns_end_kernel(const __grid_constant__ NsEnds e) {
 }
 
 // ---------------------------------------------------------------------------------------
-// matrices with a side of at most 128: a whole call in one kernel
+// matrices with a side of at most 256: a whole call in one kernel
 // ---------------------------------------------------------------------------------------
-// One cluster per matrix; each of its 1 to 16 CTAs keeps a slice of the long side (64 n columns of X, k rows) for the whole call:
+// One cluster per matrix; each of its 1 to 16 CTAs keeps a slice of the long side (64 n columns of X, RB blocks of 128 rows) for the
+// whole call:
 // the fp32 X in TMEM, its fp16 operands in shared memory. A tile of X lies as k rows of 128-byte pieces, which is the K-major
 // operand of A = X X^T and, read as rows of the reduction, the MN-major operand of B X. X in TMEM is stored times a, so that
 // the MMAs of B X add to the linear term in place (with pairs B X has columns of its own and is added in registers: the
@@ -943,21 +944,23 @@ ns_end_kernel(const __grid_constant__ NsEnds e) {
 // one 128 x 512 matrix took 111 us as tiles handed out by ns_chain_body.
 constexpr int SM_THREADS = 512;                      // 16 warps: four share the rows of a lane quarter and split its columns
 constexpr int SM_PANEL = 128 * 128;                 // 128 rows x 64 fp16
-constexpr int SM_STAGE_LD = 65;                     // fp32 staging of a panel, one word of padding a row
 
-template <bool SPLIT>
+template <int RB, bool SPLIT>
 struct SmShape {
-  static constexpr int SLICE = SPLIT ? 128 : 256;                    // columns a CTA holds at most
+  static constexpr int SLICE = RB == 2 ? 64 : (SPLIT ? 128 : 256);   // columns a CTA holds at most
   static constexpr int PLANES = SPLIT ? 2 : 1;                       // hi, lo
-  static constexpr int X_BYTES = SLICE / 64 * SM_PANEL;              // one plane of X
-  static constexpr int F_BYTES = 2 * SM_PANEL;                       // one plane of A or B
-  static constexpr int PART_BYTES = 128 * 128 * 4;                   // this CTA's share of A in fp32
-  // pairs: the shares lie where B does, which is not in use between B X and the next B
-  static constexpr int SMEM = PLANES * (X_BYTES + 2 * F_BYTES) + (SPLIT ? 0 : PART_BYTES) + 1024;
-  static constexpr int X_COL = 0, ACC_COL = SLICE;                   // TMEM columns
+  static constexpr int BLOCKS = RB * (RB + 1) / 2;                   // 128 x 128 blocks of A and B on and above the diagonal
+  static constexpr int X_BYTES = RB * SLICE / 64 * SM_PANEL;         // one plane of X
+  static constexpr int F_BYTES = 2 * SM_PANEL;                       // one plane of a block of A or B
+  static constexpr int PART_BYTES = 128 * 128 * 4;                   // this CTA's share of a block of A in fp32
+  // The shares lie where B does, which is not in use between B X and the next B (one block of B alone is too small for them).
+  static constexpr bool PART_IN_B = PLANES * BLOCKS * F_BYTES >= PART_BYTES;
+  static constexpr int SMEM = PLANES * (X_BYTES + 2 * BLOCKS * F_BYTES) + (PART_IN_B ? 0 : PART_BYTES) + 1024;
+  static constexpr int X_COL = 0, ACC_COL = RB * SLICE;              // TMEM columns
   static constexpr int BX_COL = SPLIT ? SLICE + 128 : X_COL;
   static constexpr int TMEM_COLS = 512;
 };
+static_assert(SmShape<2, false>::ACC_COL + 128 * SmShape<2, false>::BLOCKS <= 512 && SmShape<2, false>::SMEM <= 231424, "two row blocks");
 
 __device__ __forceinline__ void tmem_st_32x32(uint32_t taddr, const uint32_t (&v)[32]) {
   asm volatile(
@@ -1013,11 +1016,11 @@ __device__ __forceinline__ void sm_put_operand(uint8_t* base, int plane, int row
   }
 }
 
-// V elements an access (neighbouring along the memory's rows)
-template <bool SPLIT, int V>
+// V elements an access (neighbouring along the memory's rows). RB: blocks of 128 rows (1 or 2).
+template <int RB, bool SPLIT, int V>
 __global__ void __launch_bounds__(SM_THREADS, 1)
 ns_small_kernel(const __grid_constant__ NsEnds e, const __grid_constant__ NsSmall g, Status* status) {
-  using S = SmShape<SPLIT>;
+  using S = SmShape<RB, SPLIT>;
   extern __shared__ uint8_t smem_raw[];
   __shared__ __align__(8) uint64_t bar;
   __shared__ uint32_t tmem_slot;
@@ -1025,16 +1028,15 @@ ns_small_kernel(const __grid_constant__ NsEnds e, const __grid_constant__ NsSmal
   __shared__ double red[SM_THREADS / 32];
   __shared__ double ssq_cta;
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint8_t* xs = smem;
-  uint8_t* as = xs + S::PLANES * S::X_BYTES;
-  uint8_t* bs = as + S::PLANES * S::F_BYTES;
-  uint8_t* part = SPLIT ? bs : bs + S::F_BYTES;
-  float* staging = reinterpret_cast<float*>(part);
+  uint8_t* xs = smem;                                          // panels of 64 columns; with two row blocks one panel of each
+  uint8_t* as = xs + S::PLANES * S::X_BYTES;                   // blocks (0, 0), (0, 1), (1, 1), each with its planes
+  uint8_t* bs = as + S::PLANES * S::BLOCKS * S::F_BYTES;
+  uint8_t* part = S::PART_IN_B ? bs : bs + S::F_BYTES;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int quarter = warp & 3, part4 = warp >> 2, row = quarter * 32 + lane;
   const uint32_t ctas = g.ctas, rank = ctas > 1 ? cluster_ctarank() : 0;
   const int z = blockIdx.x / ctas;
-  const int slice = g.slice, panels = slice >> 6, s0 = (int)rank * slice;
+  const int slice = g.slice, s0 = (int)rank * slice;
   const uint32_t mma_bar = smem_u32(&bar);
 
   if (tid == 0) {
@@ -1061,58 +1063,81 @@ ns_small_kernel(const __grid_constant__ NsEnds e, const __grid_constant__ NsSmal
   const void* gt = e.grad[z];
   const void* gi = e.info[z];
   float* mom = reinterpret_cast<float*>(e.moment[z]);
-  // Element (i, j) of X is element (i, j) of the matrix, or (j, i) of a tall one; neighbouring threads take neighbouring
-  // addresses. Access n of panel p: V elements from (i, j) on, along j (along i when tall).
-  constexpr int ACCESSES = 128 * 64 / V / SM_THREADS, AT_ONCE = ACCESSES < 8 ? ACCESSES : 8;
-  auto coord = [&](int p, int n, int& i, int& j) {
-    const int t = n * SM_THREADS + tid;
-    if (g.tall) { i = t % (128 / V) * V; j = p * 64 + t / (128 / V); }
-    else { i = t / (64 / V); j = p * 64 + t % (64 / V) * V; }
-    return i < g.k && s0 + j < g.wide;
+  // Chunk c0 of X's columns in TMEM (slice columns of each row block): a thread holds row i, columns j .. j + 31 of X, which are
+  // 32 elements of a row of the matrix, or, when it is tall, of a column, where neighbouring lanes read neighbouring addresses.
+  // Sixteen elements at a time: in row-major order a lane's accesses fill whole sectors.
+  auto chunk_at = [&](int c0, int& i, int& j) {
+    i = RB == 2 ? (c0 >> 6) * 128 + row : row;
+    j = s0 + (RB == 2 ? (c0 & 63) : c0);
+  };
+  auto for_pieces = [&](int i, int j, auto body) {      // body(first element, address offset given the row pitch)
+#pragma unroll
+    for (int q = 0; q < 16 / V; ++q)
+      if (i < g.k && j + q * V < g.wide) body(q);
+  };
+  auto offset = [&](int i, int j, int64_t ld) { return g.tall ? (int64_t)j * ld + i : (int64_t)i * ld + j; };
+  auto load16 = [&](const void* p, int dtype, int64_t ld, int i, int j, float (&v)[16]) {
+    for_pieces(i, j, [&](int q) {
+      if (V > 1 && !g.tall) {
+        const VecF<V> x = load_vec<V>(p, dtype, offset(i, j + q * V, ld));
+#pragma unroll
+        for (int n = 0; n < V; ++n) v[q * V + n] = x.e[n];
+      } else {
+#pragma unroll
+        for (int n = 0; n < V; ++n)
+          if (j + q * V + n < g.wide) v[q * V + n] = load_vec<1>(p, dtype, offset(i, j + q * V + n, ld)).e[0];
+      }
+    });
+  };
+  auto store16 = [&](void* p, int dtype, int64_t ld, int i, int j, const float (&v)[16]) {
+    for_pieces(i, j, [&](int q) {
+      if (V > 1 && !g.tall) {
+        VecF<V> x;
+#pragma unroll
+        for (int n = 0; n < V; ++n) x.e[n] = v[q * V + n];
+        store_vec<V>(p, dtype, offset(i, j + q * V, ld), x);
+      } else {
+#pragma unroll
+        for (int n = 0; n < V; ++n)
+          if (j + q * V + n < g.wide) {
+            VecF<1> x;
+            x.e[0] = v[q * V + n];
+            store_vec<1>(p, dtype, offset(i, j + q * V + n, ld), x);
+          }
+      }
+    });
   };
   double ssq = 0.0;
-  for (int p = 0; p < panels; ++p) {
-#pragma unroll 1
-    for (int n0 = 0; n0 < ACCESSES; n0 += AT_ONCE) {
-      VecF<V> u[AT_ONCE], f[AT_ONCE], m[AT_ONCE];
+  for (int c0 = part4 * 32; c0 < RB * slice; c0 += 128) {
+    int i, j0;
+    chunk_at(c0, i, j0);
+    VecF<16> u[2];
 #pragma unroll
-      for (int q = 0; q < AT_ONCE; ++q) {
-        int i, j;
-        if (coord(p, n0 + q, i, j)) {
-          const int64_t r = g.tall ? s0 + j : i, c = g.tall ? i : s0 + j;
-          u[q] = load_vec<V>(gt, e.grad_dtype, r * e.grad_ld + c);
-          if (e.momentum) {
-            m[q] = *reinterpret_cast<const VecF<V>*>(mom + r * e.cols + c);
-            if (gi != nullptr) f[q] = load_vec<V>(gi, e.grad_dtype, r * e.grad_ld + c);
-          }
-        } else {
+    for (int h = 0; h < 2; ++h) {
 #pragma unroll
-          for (int x = 0; x < V; ++x) u[q].e[x] = 0.0f;
-        }
-      }
+      for (int n = 0; n < 16; ++n) u[h].e[n] = 0.0f;
+      load16(gt, e.grad_dtype, e.grad_ld, i, j0 + 16 * h, u[h].e);
+    }
+    if (e.momentum) {
 #pragma unroll
-      for (int q = 0; q < AT_ONCE; ++q) {
-        int i, j;
-        if (coord(p, n0 + q, i, j) && e.momentum) {
-          const int64_t r = g.tall ? s0 + j : i, c = g.tall ? i : s0 + j;
-          momentum_step<V>(e, kt, ki, gi != nullptr, u[q], f[q], m[q]);
-          *reinterpret_cast<VecF<V>*>(mom + r * e.cols + c) = m[q];
-        }
+      for (int h = 0; h < 2; ++h) {
+        VecF<16> f, m;
 #pragma unroll
-        for (int x = 0; x < V; ++x) staging[(i + (g.tall ? x : 0)) * SM_STAGE_LD + (j & 63) + (g.tall ? 0 : x)] = u[q].e[x];
-        add_squares<V>(ssq, u[q]);
+        for (int n = 0; n < 16; ++n) f.e[n] = m.e[n] = 0.0f;
+        if (gi != nullptr) load16(gi, e.grad_dtype, e.grad_ld, i, j0 + 16 * h, f.e);
+        load16(mom, ELEM_F32, e.cols, i, j0 + 16 * h, m.e);
+        momentum_step<16>(e, kt, ki, gi != nullptr, u[h], f, m);      // zeros outside the matrix stay zeros
+        store16(mom, ELEM_F32, e.cols, i, j0 + 16 * h, m.e);
       }
     }
-    __syncthreads();
-    if (part4 < 2) {
-      uint32_t w[32];
+    add_squares<16>(ssq, u[0]);
+    add_squares<16>(ssq, u[1]);
+    uint32_t w[32];
 #pragma unroll
-      for (int c = 0; c < 32; ++c) w[c] = __float_as_uint(staging[row * SM_STAGE_LD + part4 * 32 + c]);
-      tmem_st_32x32(tmem_row + S::X_COL + p * 64 + part4 * 32, w);
-      tmem_st_wait();
-    }
-    __syncthreads();
+    for (int n = 0; n < 32; ++n) w[n] = __float_as_uint(u[n >> 4].e[n & 15]);
+    tmem_st_32x32(tmem_row + S::X_COL + c0, w);
   }
+  tmem_st_wait();
   tc_fence_before_sync();
   double total = block_sum(ssq, red);
   if (ctas > 1) {
@@ -1150,28 +1175,29 @@ ns_small_kernel(const __grid_constant__ NsEnds e, const __grid_constant__ NsSmal
     tc_fence_after_sync();
   };
   const uint32_t xs_addr = smem_u32(xs), as_addr = smem_u32(as), bs_addr = smem_u32(bs);
-  // acc (+)= P Q^T; hi lo, lo hi, hi hi. P, Q: planes of an operand; q_mn: Q is X as the rows of the reduction
-  auto issue = [&](uint32_t acc_col, uint32_t p0, int p_plane, uint32_t q0, int q_plane, bool q_mn, int k_steps, int n, bool add) {
-    if (warp == 0 && elect_one()) {
-      const uint32_t idesc = make_instr_desc(0, 0, 0, q_mn ? 1 : 0, 128, (uint32_t)n);
-      uint32_t on = add ? 1u : 0u;
-      for (int seg = SPLIT ? 0 : 2; seg < 3; ++seg) {
-        const uint32_t pb = p0 + (seg == 1 ? p_plane : 0), qb = q0 + (seg == 0 ? q_plane : 0);
-        for (int s = 0; s < k_steps; ++s) {
-          const uint32_t k_off = (s >> 2) * SM_PANEL + (s & 3) * 32;          // K-major: 16 columns further
-          const uint64_t dp = make_smem_desc(pb + k_off, 16, 1024);
-          const uint64_t dq = q_mn ? make_smem_desc(qb + s * (16 * 128), SM_PANEL, 1024) : make_smem_desc(qb + k_off, 16, 1024);
-          mma_bf16(tmem_slot + acc_col, dp, dq, idesc, on);
-          on = 1u;
-        }
+  // One thread: acc (+)= P Q^T over k_steps x 16 of the reduction; hi lo, lo hi, hi hi. An MN-major operand lies as rows of the
+  // reduction in panels of 64 columns.
+  auto mma_run = [&](uint32_t acc_col, uint32_t p0, int p_plane, bool p_mn, uint32_t q0, int q_plane, bool q_mn, int k_steps, int n, bool add) {
+    const uint32_t idesc = make_instr_desc(0, 0, p_mn ? 1 : 0, q_mn ? 1 : 0, 128, (uint32_t)n);
+    uint32_t on = add ? 1u : 0u;
+    for (int seg = SPLIT ? 0 : 2; seg < 3; ++seg) {
+      const uint32_t pb = p0 + (seg == 1 ? p_plane : 0), qb = q0 + (seg == 0 ? q_plane : 0);
+      for (int s = 0; s < k_steps; ++s) {
+        const uint32_t k_off = (s >> 2) * SM_PANEL + (s & 3) * 32, mn_off = s * (16 * 128);
+        const uint64_t dp = p_mn ? make_smem_desc(pb + mn_off, SM_PANEL, 1024) : make_smem_desc(pb + k_off, 16, 1024);
+        const uint64_t dq = q_mn ? make_smem_desc(qb + mn_off, SM_PANEL, 1024) : make_smem_desc(qb + k_off, 16, 1024);
+        mma_bf16(tmem_slot + acc_col, dp, dq, idesc, on);
+        on = 1u;
       }
-      mma_commit(mma_bar);
     }
-    __syncwarp();
   };
+  // block (i, j) of a symmetric factor: stored at and above the diagonal, read below it in the other major order
+  auto block_of = [](int i, int j) { return i <= j ? i * (RB - 1) + j : j * (RB - 1) + i; };
+  constexpr int BLOCK_BYTES = S::PLANES * S::F_BYTES;
 
   // ---- X scaled: operands, and a X for the products to add to
-  for (int c0 = part4 * 32; c0 < slice; c0 += 128) {
+  // columns of X in TMEM: slice columns of each row block
+  for (int c0 = part4 * 32; c0 < RB * slice; c0 += 128) {
     uint32_t w[32];
     float v[32];
     tmem_ld_32x32(tmem_row + S::X_COL + c0, w);
@@ -1181,7 +1207,7 @@ ns_small_kernel(const __grid_constant__ NsEnds e, const __grid_constant__ NsSmal
       v[i] = fine ? __uint_as_float(w[i]) * finv : (float)((double)__uint_as_float(w[i]) * inv);
       w[i] = __float_as_uint(SPLIT ? v[i] : v[i] * (g.a * NS_SCALE));
     }
-    sm_put_operand<SPLIT>(xs, S::X_BYTES, row, c0, v);
+    sm_put_operand<SPLIT>(xs, S::X_BYTES, row, c0, v);      // with two row blocks c0 / 64 is the block, which is also the panel
     tmem_st_32x32(tmem_row + S::X_COL + c0, w);
   }
   tmem_st_wait();
@@ -1189,9 +1215,18 @@ ns_small_kernel(const __grid_constant__ NsEnds e, const __grid_constant__ NsSmal
   for (int step = 0; step < g.steps; ++step) {
     // A = X X^T
     publish(false);
-    issue(S::ACC_COL, xs_addr, S::X_BYTES, xs_addr, S::X_BYTES, false, slice >> 4, 128, false);
+    if (warp == 0 && elect_one()) {
+#pragma unroll
+      for (int i = 0; i < RB; ++i)
+#pragma unroll
+        for (int j = i; j < RB; ++j)
+          mma_run(S::ACC_COL + 128 * block_of(i, j), xs_addr + i * SM_PANEL, S::X_BYTES, false, xs_addr + j * SM_PANEL, S::X_BYTES, false,
+                  slice >> 4, 128, false);
+      mma_commit(mma_bar);
+    }
+    __syncwarp();
     mma_wait();
-    if (ctas == 1) {
+    if (RB == 1 && ctas == 1) {
       uint32_t w[32];
       float v[32];
       tmem_ld_32x32(tmem_row + S::ACC_COL + part4 * 32, w);
@@ -1201,9 +1236,10 @@ ns_small_kernel(const __grid_constant__ NsEnds e, const __grid_constant__ NsSmal
       sm_put_operand<SPLIT>(as, S::F_BYTES, row, part4 * 32, v);
       publish(false);
     } else {
+      for (int blk = 0; blk < S::BLOCKS; ++blk) {
       // this CTA's share as 512-byte rows of 16-byte pieces, XOR-ed with the row
       uint32_t w[32];
-      tmem_ld_32x32(tmem_row + S::ACC_COL + part4 * 32, w);
+      tmem_ld_32x32(tmem_row + S::ACC_COL + 128 * blk + part4 * 32, w);
       tmem_ld_wait();
 #pragma unroll
       for (int q = 0; q < 8; ++q)
@@ -1212,43 +1248,76 @@ ns_small_kernel(const __grid_constant__ NsEnds e, const __grid_constant__ NsSmal
       cluster_sync_all();
       // rows rank * 128 / ctas ...: sum over the CTAs, result to all of them
       const int rows_here = 128 / (int)ctas;
-      for (int t = tid; t < rows_here * 32; t += SM_THREADS) {
-        const int r = (int)rank * rows_here + (t >> 5), q = t & 31;
-        const uint32_t at = smem_u32(part + r * 512 + ((q ^ (r & 7)) << 4));
-        float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        for (uint32_t c0 = 0; c0 < ctas; c0 += 8) {
-          float4 v[8];
+      for (int t0 = tid; t0 < rows_here * 32; t0 += 2 * SM_THREADS) {      // two 16-byte pieces a thread in flight, of up to four CTAs each
+        float4 sum[2];
 #pragma unroll
-          for (uint32_t c = 0; c < 8; ++c)
-            if (c0 + c < ctas) v[c] = ld_dsmem_f4(at, c0 + c);
+        for (int h = 0; h < 2; ++h) sum[h] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        auto piece = [&](int h, int& r, int& q) {
+          const int t = t0 + h * SM_THREADS;
+          r = (int)rank * rows_here + (t >> 5);
+          q = t & 31;
+          return t < rows_here * 32;
+        };
+        for (uint32_t c0 = 0; c0 < ctas; c0 += 4) {
+          float4 v[2][4];
 #pragma unroll
-          for (uint32_t c = 0; c < 8; ++c)
-            if (c0 + c < ctas) { sum.x += v[c].x; sum.y += v[c].y; sum.z += v[c].z; sum.w += v[c].w; }
+          for (int h = 0; h < 2; ++h) {
+            int r, q;
+            const bool live = piece(h, r, q);
+            const uint32_t at = smem_u32(part + r * 512 + ((q ^ (r & 7)) << 4));
+#pragma unroll
+            for (uint32_t c = 0; c < 4; ++c)
+              if (live && c0 + c < ctas) v[h][c] = ld_dsmem_f4(at, c0 + c);
+          }
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (uint32_t c = 0; c < 4; ++c)
+              if (c0 + c < ctas) { sum[h].x += v[h][c].x; sum[h].y += v[h][c].y; sum[h].z += v[h][c].z; sum[h].w += v[h][c].w; }
         }
-        sum.x *= NS_UNSCALE; sum.y *= NS_UNSCALE; sum.z *= NS_UNSCALE; sum.w *= NS_UNSCALE;
-        const uint2 hi = make_uint2(pack_half2(sum.x, sum.y), pack_half2(sum.z, sum.w));
-        const float2 h0 = unpack_half2(hi.x), h1 = unpack_half2(hi.y);
-        const uint2 lo = make_uint2(pack_half2(sum.x - h0.x, sum.y - h0.y), pack_half2(sum.z - h1.x, sum.w - h1.y));
-        const int col = q * 4;
-        const uint32_t to = smem_u32(as + (col >> 6) * SM_PANEL + sm_piece(r, (col & 63) >> 3) + (col & 7) * 2);
-        for (uint32_t c = 0; c < ctas; ++c) {
-          st_dsmem_u2(to, c, hi);
-          if (SPLIT) st_dsmem_u2(to + S::F_BYTES, c, lo);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          int r, q;
+          if (!piece(h, r, q)) continue;
+          const float s0_ = sum[h].x * NS_UNSCALE, s1_ = sum[h].y * NS_UNSCALE, s2_ = sum[h].z * NS_UNSCALE, s3_ = sum[h].w * NS_UNSCALE;
+          const uint2 hi = make_uint2(pack_half2(s0_, s1_), pack_half2(s2_, s3_));
+          const float2 h0 = unpack_half2(hi.x), h1 = unpack_half2(hi.y);
+          const uint2 lo = make_uint2(pack_half2(s0_ - h0.x, s1_ - h0.y), pack_half2(s2_ - h1.x, s3_ - h1.y));
+          const int col = q * 4;
+          const uint32_t to = smem_u32(as + blk * BLOCK_BYTES + (col >> 6) * SM_PANEL + sm_piece(r, (col & 63) >> 3) + (col & 7) * 2);
+          for (uint32_t c = 0; c < ctas; ++c) {
+            st_dsmem_u2(to, c, hi);
+            if (SPLIT) st_dsmem_u2(to + S::F_BYTES, c, lo);
+          }
         }
       }
-      publish(true);
+      if (blk + 1 < S::BLOCKS) cluster_sync_all();      // the shares have been read
+      else publish(true);
+      }
     }
     // B = b A + c A A
-    issue(S::ACC_COL, as_addr, S::F_BYTES, as_addr, S::F_BYTES, false, 8, 128, false);
+    if (warp == 0 && elect_one()) {
+#pragma unroll
+      for (int i = 0; i < RB; ++i)
+#pragma unroll
+        for (int j = i; j < RB; ++j)
+#pragma unroll
+          for (int m = 0; m < RB; ++m)
+            mma_run(S::ACC_COL + 128 * block_of(i, j), as_addr + block_of(i, m) * BLOCK_BYTES, S::F_BYTES, i > m,
+                    as_addr + block_of(j, m) * BLOCK_BYTES, S::F_BYTES, j > m, 8, 128, m > 0);
+      mma_commit(mma_bar);
+    }
+    __syncwarp();
     mma_wait();
-    {
+#pragma unroll 1
+    for (int blk = 0; blk < S::BLOCKS; ++blk) {
       const int c0 = part4 * 32;
       uint32_t w[32];
       float v[32];
-      tmem_ld_32x32(tmem_row + S::ACC_COL + c0, w);
+      tmem_ld_32x32(tmem_row + S::ACC_COL + 128 * blk + c0, w);
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
-        const uint8_t* at = as + (c0 >> 6) * SM_PANEL + sm_piece(row, ((c0 & 63) >> 3) + q);
+        const uint8_t* at = as + blk * BLOCK_BYTES + (c0 >> 6) * SM_PANEL + sm_piece(row, ((c0 & 63) >> 3) + q);
         const uint4 hi = *reinterpret_cast<const uint4*>(at);
         const uint32_t hw[4] = {hi.x, hi.y, hi.z, hi.w};
 #pragma unroll
@@ -1269,15 +1338,24 @@ ns_small_kernel(const __grid_constant__ NsEnds e, const __grid_constant__ NsSmal
       tmem_ld_wait();
 #pragma unroll
       for (int i = 0; i < 32; ++i) v[i] = fmaf(g.b, v[i], (g.c * NS_UNSCALE) * __uint_as_float(w[i]));
-      sm_put_operand<SPLIT>(bs, S::F_BYTES, row, c0, v);
+      sm_put_operand<SPLIT>(bs + blk * BLOCK_BYTES, S::F_BYTES, row, c0, v);
     }
     publish(false);
     // X <- a X + B X
-    issue(S::BX_COL, bs_addr, S::F_BYTES, xs_addr, S::X_BYTES, true, 8, slice, !SPLIT);
+    if (warp == 0 && elect_one()) {
+#pragma unroll
+      for (int i = 0; i < RB; ++i)
+#pragma unroll
+        for (int m = 0; m < RB; ++m)
+          mma_run(S::BX_COL + i * slice, bs_addr + block_of(i, m) * BLOCK_BYTES, S::F_BYTES, i > m, xs_addr + m * SM_PANEL, S::X_BYTES, true, 8,
+                  slice, !SPLIT || m > 0);
+      mma_commit(mma_bar);
+    }
+    __syncwarp();
     mma_wait();
     if (!SPLIT && step + 1 == g.steps) break;
 #pragma unroll 1
-    for (int c0 = part4 * 32; c0 < slice; c0 += 128) {
+    for (int c0 = part4 * 32; c0 < RB * slice; c0 += 128) {
       uint32_t w[32];
       float v[32];
       tmem_ld_32x32(tmem_row + S::X_COL + c0, w);
@@ -1306,37 +1384,26 @@ ns_small_kernel(const __grid_constant__ NsEnds e, const __grid_constant__ NsSmal
 
   // ---- the result, or the parameter update
   void* out = e.out[z];
-  for (int p = 0; p < panels; ++p) {
-    if (part4 < 2) {
-      uint32_t w[32];
-      tmem_ld_32x32(tmem_row + S::X_COL + p * 64 + part4 * 32, w);
-      tmem_ld_wait();
+  for (int c0 = part4 * 32; c0 < RB * slice; c0 += 128) {
+    int i, j0;
+    chunk_at(c0, i, j0);
+    uint32_t w[32];
+    tmem_ld_32x32(tmem_row + S::X_COL + c0, w);
+    float p[2][16];
+    if (e.momentum) {
 #pragma unroll
-      for (int c = 0; c < 32; ++c) staging[row * SM_STAGE_LD + part4 * 32 + c] = __uint_as_float(w[c]) * (SPLIT ? NS_UNSCALE : NS_UNSCALE * NS_UNSCALE);
+      for (int h = 0; h < 2; ++h) load16(out, e.out_dtype, e.cols, i, j0 + 16 * h, p[h]);
     }
-    __syncthreads();
-#pragma unroll 1
-    for (int n0 = 0; n0 < ACCESSES; n0 += AT_ONCE) {
-      VecF<V> v[AT_ONCE];
+    tmem_ld_wait();
 #pragma unroll
-      for (int q = 0; q < AT_ONCE; ++q) {
-        int i, j;
-        if (!coord(p, n0 + q, i, j) || !e.momentum) continue;
-        v[q] = load_vec<V>(out, e.out_dtype, g.tall ? (int64_t)(s0 + j) * e.cols + i : (int64_t)i * e.cols + s0 + j);
+    for (int h = 0; h < 2; ++h) {
+#pragma unroll
+      for (int n = 0; n < 16; ++n) {
+        const float o = __uint_as_float(w[16 * h + n]) * (SPLIT ? NS_UNSCALE : NS_UNSCALE * NS_UNSCALE);
+        p[h][n] = e.momentum ? fmaf(-e.step, o, p[h][n] * e.decay) : o;
       }
-#pragma unroll
-      for (int q = 0; q < AT_ONCE; ++q) {
-        int i, j;
-        if (!coord(p, n0 + q, i, j)) continue;
-#pragma unroll
-        for (int x = 0; x < V; ++x) {
-          const float o = staging[(i + (g.tall ? x : 0)) * SM_STAGE_LD + (j & 63) + (g.tall ? 0 : x)];
-          v[q].e[x] = e.momentum ? fmaf(-e.step, o, v[q].e[x] * e.decay) : o;
-        }
-        store_vec<V>(out, e.out_dtype, g.tall ? (int64_t)(s0 + j) * e.cols + i : (int64_t)i * e.cols + s0 + j, v[q]);
-      }
+      store16(out, e.out_dtype, e.cols, i, j0 + 16 * h, p[h]);
     }
-    __syncthreads();
   }
 
   tc_fence_before_sync();
@@ -1419,9 +1486,9 @@ static bool ns_vec4(const NsEnds& e) {
   return vec;
 }
 
-template <bool SPLIT, int V>
-static const char* launch_small(const NsCall& call, int sms, Status* status, cudaStream_t st) {
-  using S = SmShape<SPLIT>;
+template <int RB, bool SPLIT, int V>
+static const char* launch_small(const NsCall& call, Status* status, cudaStream_t st) {
+  using S = SmShape<RB, SPLIT>;
   NsSmall g;
   g.tall = call.ends.rows > call.ends.cols;
   g.k = g.tall ? call.ends.cols : call.ends.rows;
@@ -1434,7 +1501,7 @@ static const char* launch_small(const NsCall& call, int sms, Status* status, cud
   // As few CTAs as hold the matrix: one 128 x 512 matrix takes 50 us on 2 CTAs and 43 us on 8, 48 of them 51 and 168 us.
   while (g.ctas * S::SLICE < g.wide) g.ctas *= 2;
   g.slice = ((g.wide + g.ctas - 1) / g.ctas + 63) / 64 * 64;
-  auto kernel = ns_small_kernel<SPLIT, V>;
+  auto kernel = ns_small_kernel<RB, SPLIT, V>;
   if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM) != cudaSuccess) return "orthogonalize: shared memory";
   if (g.ctas > 8 && cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess)
     return "orthogonalize: cluster size";
@@ -1452,14 +1519,22 @@ static const char* launch_small(const NsCall& call, int sms, Status* status, cud
   return cudaLaunchKernelEx(&cfg, kernel, call.ends, g, status) == cudaSuccess ? nullptr : "ns_small launch failed";
 }
 
-// A side of at most 128 and a long side of at most 2048: 8 CTAs with slices of 256 columns, 16 with slices of 128.
-static bool ns_is_small(int64_t rows, int64_t cols, int steps, int pairs) {
+// Row blocks of a matrix that one cluster keeps, 0 for the others. One block of 128 rows: 8 CTAs with slices of 256 columns, or, with
+// pairs, 16 with slices of 128. Two blocks: 4 or 8 CTAs with slices of 64 columns; pairs do not fit.
+// With two blocks the exchange of A weighs more, so they are worth it only while all clusters run at once (fewer of the larger ones
+// do): 32 matrices of 256 x 256 (4 CTAs each) 101 us against 143 in ns_chain_body, 64 of them 198 against 163; 8 of 256 x 512
+// (8 CTAs) 112 against 133, 16 of them 221 against 143; 8 of 200 x 1000 (16 CTAs) 252 against 145.
+static int ns_small_blocks(int64_t batch, int64_t rows, int64_t cols, int steps, int pairs) {
   const int64_t k = rows < cols ? rows : cols, wide = rows < cols ? cols : rows;
-  return steps > 0 && k <= 128 && wide <= (pairs ? 16 * SmShape<true>::SLICE : 8 * SmShape<false>::SLICE);
+  if (steps == 0) return 0;
+  if (k <= 128 && wide <= 2048) return 1;
+  int64_t ctas = 1;
+  while (ctas * 64 < wide) ctas *= 2;
+  return k <= 256 && !pairs && ((ctas <= 4 && batch * ctas <= 128) || (ctas == 8 && batch <= 8)) ? 2 : 0;
 }
 
 int64_t ns_workspace_bytes(int64_t batch, int64_t rows, int64_t cols, int steps, int pairs) {
-  return ns_is_small(rows, cols, steps, pairs) ? 0 : ns_space(batch, rows, cols).total;
+  return ns_small_blocks(batch, rows, cols, steps, pairs) != 0 ? 0 : ns_space(batch, rows, cols).total;
 }
 
 const char* launch_orthogonalize(const NsCall& call, Status* status, cudaStream_t st) {
@@ -1470,9 +1545,12 @@ const char* launch_orthogonalize(const NsCall& call, Status* status, cudaStream_
   if (cudaGetDevice(&dev) != cudaSuccess || cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess)
     return "orthogonalize: device";
   const bool vec = ns_vec4(call.ends);
-  if (ns_is_small(rows, cols, call.steps, call.pairs)) {
-    if (call.pairs) return vec ? launch_small<true, 4>(call, sms, status, st) : launch_small<true, 1>(call, sms, status, st);
-    return vec ? launch_small<false, 4>(call, sms, status, st) : launch_small<false, 1>(call, sms, status, st);
+  switch (ns_small_blocks(batch, rows, cols, call.steps, call.pairs)) {
+    case 1:
+      if (call.pairs) return vec ? launch_small<1, true, 4>(call, status, st) : launch_small<1, true, 1>(call, status, st);
+      return vec ? launch_small<1, false, 4>(call, status, st) : launch_small<1, false, 1>(call, status, st);
+    case 2: return vec ? launch_small<2, false, 4>(call, status, st) : launch_small<2, false, 1>(call, status, st);
+    default: break;
   }
   const NsSpace w = ns_space(batch, rows, cols);
   __half* base = reinterpret_cast<__half*>(call.workspace);

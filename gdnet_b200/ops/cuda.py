@@ -15,7 +15,6 @@ copies cached per parameter version.
 
 from __future__ import annotations
 
-import math
 import os
 import weakref
 
@@ -817,28 +816,14 @@ def embedding_grad(tokens, grad, num_rows: int, scale: float = 1.0, out=None):
 # Newton-Schulz products: orthogonalised matrices and the momentum update built on them
 # --------------------------------------------------------------------------------------
 def orthogonalize(x, steps, coefficients, eps, out_dtype, pairs):
-    r, c = x.shape[-2:]
-    x3 = x.detach().reshape(math.prod(x.shape[:-2]), r, c)
-    if x3.stride(-1) != 1 and c != 1:
-        x3 = x3.contiguous()
-    out = torch.empty(x3.shape, dtype=out_dtype, device=x.device)
-    K.orthogonalize(x3, out, steps, coefficients, eps, pairs)
-    return out.view(x.shape)
+    return K.orthogonalize(x, out_dtype, steps, coefficients, eps, pairs)
 
 
 def muon_update_(params, grads, momenta, infos, scalars, *, lr, momentum, nesterov, weight_decay, steps, coefficients, eps,
                  update_scale, beta):
-    """Matrices of one shape and type share their launches (arguments checked by the caller)."""
-    groups: dict[tuple, tuple] = {}
-    for i, p in enumerate(params):
-        lists = groups.setdefault((p.shape[-2:], p.dtype, grads[i].dtype), ([], [], [], []))
-        for to, t in zip(lists, (p, grads[i], momenta[i]) + ((infos[i],) if infos else ())):
-            to.extend(t.detach().unbind(0) if t.dim() == 3 else (t.detach(),))
-    for ((r, c), dtype, _), (ps, gs, ms, gi) in groups.items():
-        size = 0.2 * max(r, c) ** 0.5 if update_scale is None else float(update_scale)
-        K.muon_update(ps, gs, gi, ms, scalars, beta, momentum, nesterov, 1.0 - lr * weight_decay, lr * size, steps, coefficients, eps,
-                      dtype != BF16)
-    torch.autograd.graph.increment_version(params + momenta)
+    """The entries are checked and grouped by shape in the binding."""
+    K.muon_update(params, grads, infos, momenta, scalars, beta, momentum, nesterov, lr, weight_decay,
+                  -1.0 if update_scale is None else update_scale, steps, coefficients, eps)
 
 
 # --------------------------------------------------------------------------------------

@@ -21,10 +21,16 @@ def _on_gpu(t: torch.Tensor) -> bool:
     return t.is_cuda
 
 
-def _cuda():
-    from . import cuda as cuda_ops  # deferred: needs the compiled extension
+_cuda_ops = None
 
-    return cuda_ops
+
+def _cuda():
+    global _cuda_ops
+    if _cuda_ops is None:
+        from . import cuda  # deferred: needs the compiled extension
+
+        _cuda_ops = cuda
+    return _cuda_ops
 
 
 # --------------------------------------------------------------------------------------
@@ -107,7 +113,7 @@ def embedding(tokens, weight, scale: float = 1.0):
     if weight.dim() != 2 or weight.dtype not in _TABLE_TYPES:
         raise TypeError(f"embedding: the table must be a bf16, fp16 or fp32 matrix, got {weight.dtype} {tuple(weight.shape)}")
     _check_tokens(tokens, weight, "embedding")
-    if _on_gpu(weight):
+    if weight.is_cuda:
         return _cuda().embedding(tokens, weight, float(scale))
     return ref.embedding(tokens, weight, float(scale))
 
@@ -162,6 +168,8 @@ def _ns_check(coefficients: tuple, steps: int) -> None:
 
 
 def _ns_arguments(steps, coefficients, eps, what: str):
+    if steps == 5 and coefficients is NS_COEFFICIENTS and eps == 1e-7:      # the defaults
+        return steps, coefficients, eps
     steps, eps = int(steps), float(eps)
     coefficients = tuple(float(x) for x in coefficients)
     if not 0 <= steps <= 100:
@@ -236,6 +244,13 @@ def muon_update_(params, grads, momenta, *, lr: float, momentum: float = 0.95, n
     dev = params[0].device
     if scalars is not None and (scalars.dtype != torch.float32 or scalars.numel() < 2 or scalars.device != dev):
         raise ValueError("muon_update_: scalars must be two fp32 values on the params' device")
+    if update_scale is not None and not update_scale >= 0.0:
+        raise ValueError(f"muon_update_: update_scale must not be negative, got {update_scale}")
+    if dev.type == "cuda":      # the entries' own checks are made where they are gathered, in the binding
+        _cuda().muon_update_(params, grads, momenta, infos, scalars, lr=float(lr), momentum=float(momentum), nesterov=bool(nesterov),
+                             weight_decay=float(weight_decay), steps=steps, coefficients=coefficients, eps=eps,
+                             update_scale=update_scale, beta=float(beta))
+        return
     for i, p in enumerate(params):
         mine = [p, grads[i], momenta[i]] + ([infos[i]] if infos else [])
         if p.dim() not in (2, 3) or any(t.shape != p.shape for t in mine):
@@ -248,11 +263,6 @@ def muon_update_(params, grads, momenta, *, lr: float, momentum: float = 0.95, n
             raise TypeError(f"muon_update_: entry {i} has gradients of two types")
     if _overlap(params + momenta, grads + infos):
         raise ValueError("muon_update_: entries share memory")
-    hyper = dict(lr=float(lr), momentum=float(momentum), nesterov=bool(nesterov), weight_decay=float(weight_decay),
-                 steps=steps, coefficients=coefficients, eps=eps, update_scale=update_scale, beta=float(beta))
-    if dev.type == "cuda":
-        _cuda().muon_update_(params, grads, momenta, infos, scalars, **hyper)
-        return
     for i, p in enumerate(params):
         g = grads[i].float()
         if scalars is not None:

@@ -133,7 +133,7 @@ def test_muon_reference_and_refusals():
     for kw in (dict(gs=[]), dict(ps=[torch.ones(4)], gs=[torch.ones(4)], ms=[torch.ones(4)]), dict(gs=[torch.ones(4, 5)]),
                dict(ps=[torch.ones(4, 8)[:, ::2]]), dict(ps=[t], gs=[t]), dict(ps=[t], ms=[t]), dict(steps=200),
                dict(ps=[t, t], gs=[torch.ones(4, 4)] * 2, ms=[torch.ones(4, 4), torch.ones(4, 4)]),
-               dict(info_grads=[torch.ones(4, 4)]), dict(scalars=torch.ones(1)), dict(scalars=torch.ones(2, dtype=torch.float64))):
+               dict(info_grads=[torch.ones(4, 4)]), dict(update_scale=-1.0), dict(scalars=torch.ones(1)), dict(scalars=torch.ones(2, dtype=torch.float64))):
         with pytest.raises(ValueError):
             call(**kw)
     flat = torch.ones(40)
