@@ -1078,13 +1078,13 @@ int elem_type(const Tensor& t, const char* name) {
     case at::kBFloat16: return gd::ELEM_BF16;
     case at::kHalf: return gd::ELEM_F16;
     case at::kFloat: return gd::ELEM_F32;
-    default: TORCH_CHECK(false, name, " must be bfloat16, float16 or float32");
+    default: TORCH_CHECK_TYPE(false, name, " must be bfloat16, float16 or float32");
   }
 }
 
 void check_tokens(const Tensor& tokens, const Tensor& like) {
-  TORCH_CHECK(tokens.is_cuda() && tokens.device() == like.device(), "tokens must be on the same CUDA device");
-  TORCH_CHECK(tokens.scalar_type() == at::kLong || tokens.scalar_type() == at::kInt, "tokens must be int64 or int32");
+  TORCH_CHECK_VALUE(tokens.is_cuda() && tokens.device() == like.device(), "tokens must be on the same CUDA device");
+  TORCH_CHECK_TYPE(tokens.scalar_type() == at::kLong || tokens.scalar_type() == at::kInt, "tokens must be int64 or int32");
   TORCH_CHECK(tokens.is_contiguous(), "tokens must be contiguous");
 }
 
@@ -1093,7 +1093,7 @@ Tensor token_lookup(const Tensor& tokens, const Tensor& table, double scale) {
   OpRange gd_range_(__func__);
   check_cuda(table, "table");
   check_tokens(tokens, table);
-  TORCH_CHECK(table.dim() == 2, "token_lookup: the table is a matrix");
+  TORCH_CHECK_TYPE(table.dim() == 2, "token_lookup: the table is a matrix");
   std::vector<int64_t> shape(tokens.sizes().begin(), tokens.sizes().end());
   shape.push_back(table.size(1));
   Tensor out = at::empty(shape, table.options());

@@ -72,30 +72,32 @@ constexpr int NS_BK = 64;                       // K elements per stage: one 128
 constexpr int NS_EPI_WARPS = 8;
 constexpr int NS_THREADS = 96 + NS_EPI_WARPS * 32;
 constexpr int NS_OPERAND_BYTES = 128 * 128;     // 128 rows x 64 fp16 per CTA and operand
-constexpr int NS_STAGE_BYTES = 2 * NS_OPERAND_BYTES;
 constexpr int NS_BOX = 32;                      // epilogue chunk: 32 x 32
 constexpr int NS_BOX_BYTES = NS_BOX * NS_BOX * 2;
 constexpr int NS_SLOTS = 2;                     // chunks of the linear term in flight per epilogue warp
-constexpr int NS_ACC = 2;
-constexpr int NS_SPLIT_KBLOCKS = 2;             // pairs: K blocks summed in TMEM before the sum moves to registers
+constexpr int NS_MAX_ACC = 4;
 // Items on their way through a block: two are handed out ahead of the loads, which run at most the stages (4) ahead of the
 // MMAs, these two accumulators ahead of the epilogue; a ring of 16 is never overwritten before it is read.
 constexpr int NS_RING = 16;
 
 template <bool SPLIT>
 struct NsShape {
-  static constexpr int STAGES = 4;
+  static constexpr int PLANES = SPLIT ? 2 : 1;                                // hi, lo: a stage holds both of both operands
+  static constexpr int STAGES = SPLIT ? 2 : 4;
+  static constexpr int P_BYTES = PLANES * NS_OPERAND_BYTES;
+  static constexpr int STAGE_BYTES = 2 * P_BYTES;
+  static constexpr int ACC = SPLIT ? 4 : 2;                                   // accumulators in TMEM; with pairs they change hands more often
   static constexpr int AUX_BYTES = 2 * NS_BOX_BYTES;                          // hi and lo
   static constexpr int OUT_BYTES = 2 * NS_BOX_BYTES;
   static constexpr int WARP_BYTES = NS_SLOTS * AUX_BYTES + OUT_BYTES;
-  static constexpr int SMEM = STAGES * NS_STAGE_BYTES + NS_EPI_WARPS * WARP_BYTES + 1024 + 1024;   // barriers; alignment
+  static constexpr int SMEM = STAGES * STAGE_BYTES + NS_EPI_WARPS * WARP_BYTES + 1024 + 1024;   // barriers; alignment
 };
 
 struct __align__(16) NsBars {
   uint64_t full[4];
   uint64_t empty[4];
-  uint64_t acc_full[NS_ACC];
-  uint64_t acc_empty[NS_ACC];
+  uint64_t acc_full[NS_MAX_ACC];
+  uint64_t acc_empty[NS_MAX_ACC];
   uint64_t aux_full[NS_EPI_WARPS * NS_SLOTS];
   uint64_t item_full[NS_RING];
   uint64_t taken[2];                 // the loads have begun item it (barrier it & 1)
@@ -247,12 +249,12 @@ template <bool PAIR, bool SPLIT>
 __device__ __forceinline__ void ns_chain_body(const NsPlan& g, Status* status) {
   constexpr int TILE = PAIR ? 256 : 128;
   constexpr int CHUNKS = TILE / 64;              // 32-column chunks per epilogue warp (two warps share a lane quarter)
-  constexpr int SEGS = SPLIT ? 3 : 1;
-  constexpr int STAGES = NsShape<SPLIT>::STAGES;
+  constexpr int STAGES = NsShape<SPLIT>::STAGES, ACC = NsShape<SPLIT>::ACC, PLANES = NsShape<SPLIT>::PLANES;
+  constexpr int P_BYTES = NsShape<SPLIT>::P_BYTES, STAGE_BYTES = NsShape<SPLIT>::STAGE_BYTES;
   constexpr uint32_t WARPS_PER_TILE = (PAIR ? 2 : 1) * NS_EPI_WARPS;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint8_t* boxes = smem + STAGES * NS_STAGE_BYTES;
+  uint8_t* boxes = smem + STAGES * STAGE_BYTES;
   NsBars* bars = reinterpret_cast<NsBars*>(boxes + NS_EPI_WARPS * NsShape<SPLIT>::WARP_BYTES);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = PAIR ? cluster_ctarank() : 0;
@@ -262,7 +264,7 @@ __device__ __forceinline__ void ns_chain_body(const NsPlan& g, Status* status) {
       mbar_init(smem_u32(&bars->full[s]), 1);
       mbar_init(smem_u32(&bars->empty[s]), 1);
     }
-    for (int a = 0; a < NS_ACC; ++a) {
+    for (int a = 0; a < ACC; ++a) {
       mbar_init(smem_u32(&bars->acc_full[a]), 1);
       mbar_init(smem_u32(&bars->acc_empty[a]), WARPS_PER_TILE);
     }
@@ -278,8 +280,8 @@ __device__ __forceinline__ void ns_chain_body(const NsPlan& g, Status* status) {
     for (int i = (warp - 2) * 32 + lane; i < (int)(NS_MAPS); i += (NS_THREADS - 64)) tma_prefetch_desc(maps + i);
   }
   if (warp == 1) {
-    if (PAIR) { tmem_alloc_pair(smem_u32(&bars->tmem_base), NS_ACC * TILE); tmem_relinquish_pair(); }
-    else { tmem_alloc(smem_u32(&bars->tmem_base), NS_ACC * TILE); tmem_relinquish(); }
+    if (PAIR) { tmem_alloc_pair(smem_u32(&bars->tmem_base), ACC * TILE); tmem_relinquish_pair(); }
+    else { tmem_alloc(smem_u32(&bars->tmem_base), ACC * TILE); tmem_relinquish(); }
   }
   tc_fence_before_sync();
   __syncthreads();
@@ -306,58 +308,57 @@ __device__ __forceinline__ void ns_chain_body(const NsPlan& g, Status* status) {
       const int cur = t.step & 1;
       const int m0 = t.mb * TILE + (int)rank * 128, n0 = t.nb * TILE + (int)rank * 128;
       const int kblocks = t.phase == 0 ? kb_x : kb_k;
-      for (int seg = 0; seg < SEGS && ok; ++seg) {
-        // hi lo, lo hi, hi hi: the small partial products first
-        const int p_lo = (SPLIT && seg == 1) ? 1 : 0, q_lo = (SPLIT && seg == 0) ? 1 : 0;
-        const bool once = t.phase != 2 && t.mb == t.nb && p_lo == q_lo;      // both operands are the same rows
-        // the symmetric factor (A, or B) and, but for B = b A + c A A, the X operand
-        const CUtensorMap* fp = t.phase == 1 ? g.a_load[p_lo] : g.b_load[p_lo];
-        const CUtensorMap* fq = t.phase == 1 ? g.a_load[q_lo] : g.b_load[q_lo];
-        const CUtensorMap* xp = t.phase == 0 ? &g.x_gram[cur][p_lo] : &g.x_apply[cur][p_lo];
-        const CUtensorMap* xq = t.phase == 0 ? &g.x_gram[cur][q_lo] : &g.x_apply[cur][q_lo];
-        for (int kb = 0, kx = 0; kb < kblocks; ++kb, kx += NS_BK) {
-          if (!__all_sync(0xffffffffu, ns_wait(empty0 + 8 * s, ph ^ 1))) {
-            if (lane == 0) ns_abort(bars, status, STATUS_TIMEOUT_SMEM_EMPTY, 80, s);
-            ok = false;
-            break;
-          }
-          const uint32_t full = full_lead0 + 8 * s;
-          const uint32_t p_dst = smem0 + s * NS_STAGE_BYTES, q_dst = p_dst + NS_OPERAND_BYTES;
-          if (elect_one()) {
-            if (!PAIR || rank == 0) mbar_arrive_expect_tx(full0 + 8 * s, (PAIR ? 2 : 1) * (once ? NS_OPERAND_BYTES : NS_STAGE_BYTES));
-            auto load = [&](uint32_t dst, const CUtensorMap* m, bool mn, int row) {      // rows row .. row + 127, this K block
-              auto copy = [&](uint32_t d, int x, int y) {
-                if (PAIR) tma_load_3d_pair(d, m, full, x, y, t.z);
-                else tma_load_3d(d, m, full, x, y, t.z);
-              };
-              if (!mn) {
-                copy(dst, kx, row);
-              } else {
-#pragma unroll
-                for (int i = 0; i < 2; ++i) copy(dst + i * (NS_BK * 128), row + i * 64, kx);
-              }
-            };
-            auto factor = [&](uint32_t dst, const CUtensorMap* m, int block, int row) {
-              const bool mn = ns_below<TILE>(kb, block);
-              load(dst, &m[mn], mn, row);
-            };
-            if (t.phase == 0) {
-              load(p_dst, xp, g.tall, m0);
-              if (!once) load(q_dst, xq, g.tall, n0);
-            } else if (t.phase == 1) {
-              factor(p_dst, fp, t.mb, m0);
-              if (!once) factor(q_dst, fq, t.nb, n0);
-            } else if (g.tall) {
-              load(p_dst, xp, false, m0);
-              factor(q_dst, fq, t.nb, n0);
-            } else {
-              factor(p_dst, fp, t.mb, m0);
-              load(q_dst, xq, true, n0);
-            }
-          }
-          __syncwarp();
-          if (++s == STAGES) { s = 0; ph ^= 1; }
+      const bool once = t.phase != 2 && t.mb == t.nb;      // both operands are the same rows
+      // the symmetric factor (A, or B) [plane][major order] and, but for B = b A + c A A, the X operand [plane]
+      const CUtensorMap (*f)[2] = t.phase == 1 ? g.a_load : g.b_load;
+      const CUtensorMap* x = t.phase == 0 ? g.x_gram[cur] : g.x_apply[cur];
+      for (int kb = 0, kx = 0; kb < kblocks; ++kb, kx += NS_BK) {
+        if (!__all_sync(0xffffffffu, ns_wait(empty0 + 8 * s, ph ^ 1))) {
+          if (lane == 0) ns_abort(bars, status, STATUS_TIMEOUT_SMEM_EMPTY, 80, s);
+          ok = false;
+          break;
         }
+        const uint32_t full = full_lead0 + 8 * s;
+        const uint32_t p_dst = smem0 + s * STAGE_BYTES, q_dst = p_dst + P_BYTES;
+        if (elect_one()) {
+          if (!PAIR || rank == 0) mbar_arrive_expect_tx(full0 + 8 * s, (PAIR ? 2 : 1) * (once ? P_BYTES : STAGE_BYTES));
+          auto load = [&](uint32_t dst, const CUtensorMap* m, bool mn, int row) {      // rows row .. row + 127, this K block
+            auto copy = [&](uint32_t d, int x, int y) {
+              if (PAIR) tma_load_3d_pair(d, m, full, x, y, t.z);
+              else tma_load_3d(d, m, full, x, y, t.z);
+            };
+            if (!mn) {
+              copy(dst, kx, row);
+            } else {
+#pragma unroll
+              for (int i = 0; i < 2; ++i) copy(dst + i * (NS_BK * 128), row + i * 64, kx);
+            }
+          };
+          auto factor = [&](uint32_t dst, int block, int row) {
+            const bool mn = ns_below<TILE>(kb, block);
+#pragma unroll
+            for (int pl = 0; pl < PLANES; ++pl) load(dst + pl * NS_OPERAND_BYTES, &f[pl][mn], mn, row);
+          };
+          auto x_rows = [&](uint32_t dst, bool mn, int row) {
+#pragma unroll
+            for (int pl = 0; pl < PLANES; ++pl) load(dst + pl * NS_OPERAND_BYTES, &x[pl], mn, row);
+          };
+          if (t.phase == 0) {
+            x_rows(p_dst, g.tall, m0);
+            if (!once) x_rows(q_dst, g.tall, n0);
+          } else if (t.phase == 1) {
+            factor(p_dst, t.mb, m0);
+            if (!once) factor(q_dst, t.nb, n0);
+          } else if (g.tall) {
+            x_rows(p_dst, false, m0);
+            factor(q_dst, t.nb, n0);
+          } else {
+            factor(p_dst, t.mb, m0);
+            x_rows(q_dst, true, n0);
+          }
+        }
+        __syncwarp();
+        if (++s == STAGES) { s = 0; ph ^= 1; }
       }
     }
   } else if (warp == 1) {
@@ -370,11 +371,14 @@ __device__ __forceinline__ void ns_chain_body(const NsPlan& g, Status* status) {
         if (!t.live) break;
         const int kblocks = t.phase == 0 ? kb_x : kb_k;
         const bool diagonal = t.phase != 2 && t.mb == t.nb;
+        // An operand is MN-major for its first K blocks: X all the way or not at all, a symmetric factor up to the diagonal.
+        constexpr int ALL = 0x7fffffff, PER_TILE = TILE / NS_BK;
+        const int p_mn_until = t.phase == 0 ? (g.tall ? ALL : 0) : (t.phase == 2 && g.tall ? 0 : t.mb * PER_TILE);
+        const int q_mn_until = t.phase == 0 ? (g.tall ? ALL : 0) : (t.phase == 2 && !g.tall ? ALL : t.nb * PER_TILE);
         const uint64_t k_tmpl = make_smem_desc(smem0, 16, 1024), mn_tmpl = make_smem_desc(smem0, NS_BK * 128, 1024);
-        const int blocks = kblocks * SEGS;
-        // K blocks that one accumulator takes: all of them, or, with pairs, few enough for the sum to stay as exact as fp32
-        const int per_acc = SPLIT ? NS_SPLIT_KBLOCKS : blocks;
-        for (int b0 = 0; b0 < blocks && ok; b0 += per_acc) {
+        // K blocks that one accumulator takes: all of them, or, with pairs, one, for the sum to stay as exact as fp32
+        const int per_acc = SPLIT ? 1 : kblocks;
+        for (int b0 = 0; b0 < kblocks && ok; b0 += per_acc) {
           if (!__all_sync(0xffffffffu, ns_wait(aempty0 + 8 * acc, acc_ph ^ 1))) {
             if (lane == 0) ns_abort(bars, status, STATUS_TIMEOUT_TMEM_EMPTY, 81, acc);
             ok = false;
@@ -382,9 +386,8 @@ __device__ __forceinline__ void ns_chain_body(const NsPlan& g, Status* status) {
           }
           tc_fence_after_sync();
           const uint32_t d_tmem = tmem_base + acc * TILE;
-          const int count = min(per_acc, blocks - b0);
+          const int count = min(per_acc, kblocks - b0);
           uint32_t accumulate = 0;
-          int kb = b0 % kblocks;
           for (int i = 0; i < count; ++i) {
             if (!__all_sync(0xffffffffu, ns_wait(full0 + 8 * s, ph))) {
               if (lane == 0) ns_abort(bars, status, STATUS_TIMEOUT_SMEM_FULL, 82, s);
@@ -392,24 +395,23 @@ __device__ __forceinline__ void ns_chain_body(const NsPlan& g, Status* status) {
               break;
             }
             tc_fence_after_sync();
-            // major order of this K block's operands
-            const bool p_mn = t.phase == 0 ? g.tall : (t.phase == 1 || !g.tall) && ns_below<TILE>(kb, t.mb);
-            const bool q_mn = t.phase == 0 ? g.tall : (t.phase == 2 && !g.tall) || ns_below<TILE>(kb, t.nb);
-            const uint32_t idesc = make_instr_desc(0, 0, p_mn ? 1 : 0, q_mn ? 1 : 0, TILE, TILE);
+            const bool p_mn = b0 + i < p_mn_until, q_mn = b0 + i < q_mn_until;
+            const uint32_t idesc = make_instr_desc(0, 0, 0, 0, TILE, TILE) | (p_mn ? 1u << 15 : 0u) | (q_mn ? 1u << 16 : 0u);
             const uint32_t p_step = p_mn ? (16 * 128) >> 4 : 2, q_step = q_mn ? (16 * 128) >> 4 : 2;
-            const bool once = diagonal && (!SPLIT || b0 + i >= 2 * kblocks);     // hi hi comes last
-            const uint64_t p_tmpl = p_mn ? mn_tmpl : k_tmpl, q_tmpl = q_mn ? mn_tmpl : k_tmpl;
-            const uint32_t p_hi = (uint32_t)(p_tmpl >> 32), q_hi = (uint32_t)(q_tmpl >> 32);
-            const uint32_t p_lo = (uint32_t)p_tmpl + s * (NS_STAGE_BYTES >> 4);
-            const uint32_t q_lo = (uint32_t)q_tmpl + s * (NS_STAGE_BYTES >> 4) + (once ? 0 : NS_OPERAND_BYTES >> 4);
-            if (++kb == kblocks) kb = 0;
+            const uint32_t d_hi = (uint32_t)(k_tmpl >> 32);                       // the strides that differ are in the low word
+            const uint32_t p_lo = (uint32_t)(p_mn ? mn_tmpl : k_tmpl) + s * (STAGE_BYTES >> 4);
+            const uint32_t q_lo = (uint32_t)(q_mn ? mn_tmpl : k_tmpl) + s * (STAGE_BYTES >> 4) + (diagonal ? 0 : P_BYTES >> 4);
             if (elect_one()) {
 #pragma unroll
-              for (int k = 0; k < NS_BK / 16; ++k) {
-                const uint64_t dp = ns_desc(p_hi, p_lo + k * p_step), dq = ns_desc(q_hi, q_lo + k * q_step);
-                const uint32_t on = k == 0 ? accumulate : 1u;
-                if (PAIR) mma_bf16_pair(d_tmem, dp, dq, idesc, on);      // kind::f16; idesc says fp16
-                else mma_bf16(d_tmem, dp, dq, idesc, on);
+              for (int part = SPLIT ? 0 : 2; part < 3; ++part) {                 // hi lo, lo hi, hi hi
+                const uint32_t p_at = p_lo + (part == 1 ? NS_OPERAND_BYTES >> 4 : 0), q_at = q_lo + (part == 0 ? NS_OPERAND_BYTES >> 4 : 0);
+#pragma unroll
+                for (int k = 0; k < NS_BK / 16; ++k) {
+                  const uint64_t dp = ns_desc(d_hi, p_at + k * p_step), dq = ns_desc(d_hi, q_at + k * q_step);
+                  const uint32_t on = k == 0 && part == (SPLIT ? 0 : 2) ? accumulate : 1u;
+                  if (PAIR) mma_bf16_pair(d_tmem, dp, dq, idesc, on);      // kind::f16; idesc says fp16
+                  else mma_bf16(d_tmem, dp, dq, idesc, on);
+                }
               }
               if (PAIR) mma_commit_pair(empty0 + 8 * s);
               else mma_commit(empty0 + 8 * s);
@@ -424,7 +426,7 @@ __device__ __forceinline__ void ns_chain_body(const NsPlan& g, Status* status) {
             else mma_commit(afull0 + 8 * acc);
           }
           __syncwarp();
-          if (++acc == NS_ACC) { acc = 0; acc_ph ^= 1; }
+          if (++acc == ACC) { acc = 0; acc_ph ^= 1; }
         }
       }
     }
@@ -537,7 +539,7 @@ __device__ __forceinline__ void ns_chain_body(const NsPlan& g, Status* status) {
           if (PAIR) mbar_arrive_cluster(aempty_lead0 + 8 * acc);
           else mbar_arrive(aempty0 + 8 * acc);
         }
-        if (++acc == NS_ACC) { acc = 0; acc_ph ^= 1; }
+        if (++acc == ACC) { acc = 0; acc_ph ^= 1; }
       };
       auto acc_row = [&]() { return tmem_base + ((uint32_t)(quarter * 32) << 16) + acc * TILE + half * (TILE / 2); };
 
@@ -610,14 +612,14 @@ __device__ __forceinline__ void ns_chain_body(const NsPlan& g, Status* status) {
 
       if constexpr (SPLIT) {
         // Pairs: the tensor core cuts a running sum where fp32 rounds it, an error of one sign that grows with the number of
-        // additions, so every few K blocks the sum moves to registers and is continued there.
+        // additions, so after every K block the sum moves to registers and is continued there.
         float sum[CHUNKS][32];
 #pragma unroll
         for (int c = 0; c < CHUNKS; ++c)
 #pragma unroll
           for (int j = 0; j < 32; ++j) sum[c][j] = 0.0f;
-        const int blocks = (t.phase == 0 ? kb_x : kb_k) * SEGS;
-        for (int b0 = 0; b0 < blocks && ok; b0 += NS_SPLIT_KBLOCKS) {
+        const int kblocks = t.phase == 0 ? kb_x : kb_k;
+        for (int b0 = 0; b0 < kblocks && ok; ++b0) {
           if (!(ok = acc_wait())) break;
 #pragma unroll
           for (int c = 0; c < CHUNKS; ++c) {
@@ -696,8 +698,8 @@ __device__ __forceinline__ void ns_chain_body(const NsPlan& g, Status* status) {
   if (PAIR) cluster_sync_all();
   if (warp == 1) {
     tc_fence_after_sync();
-    if (PAIR) tmem_dealloc_pair(tmem_base, NS_ACC * TILE);
-    else tmem_dealloc(tmem_base, NS_ACC * TILE);
+    if (PAIR) tmem_dealloc_pair(tmem_base, ACC * TILE);
+    else tmem_dealloc(tmem_base, ACC * TILE);
   }
 }
 

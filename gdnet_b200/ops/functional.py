@@ -110,11 +110,11 @@ def embedding(tokens, weight, scale: float = 1.0):
     Differentiable in ``weight``. On CUDA the gradient is :func:`embedding_grad`: with a ``main_grad`` installed by the
     training engine it is added there in fp32 and autograd gets none. An id outside the table gives a row of zeros, no
     gradient, and a bad-argument code in the kernel status word (on CPU an ``IndexError``)."""
+    if weight.is_cuda:      # checked in the binding
+        return _cuda().embedding(tokens, weight, scale)
     if weight.dim() != 2 or weight.dtype not in _TABLE_TYPES:
         raise TypeError(f"embedding: the table must be a bf16, fp16 or fp32 matrix, got {weight.dtype} {tuple(weight.shape)}")
     _check_tokens(tokens, weight, "embedding")
-    if weight.is_cuda:
-        return _cuda().embedding(tokens, weight, float(scale))
     return ref.embedding(tokens, weight, float(scale))
 
 

@@ -175,3 +175,24 @@ def test_large_list_and_offsets_past_32_bits():
     assert torch.equal(got, want[:, None].expand(5, width))
     y = ops.embedding(tok, torch.arange(5, dtype=BF, device=DEV)[:, None].expand(5, width).contiguous())
     assert torch.equal(y[:, 0].long(), tok) and torch.equal(y[:, -1].long(), tok)
+
+
+def test_refusals():
+    """Arguments that the binding refuses before anything is launched."""
+    w, tok = torch.ones(5, 3, device=DEV), torch.zeros(4, dtype=torch.int64, device=DEV)
+    for bad in (w.double(), w[0], w.int()):
+        with pytest.raises(TypeError):
+            ops.embedding(tok, bad)
+    for t in (tok.float(), tok.bool()):
+        with pytest.raises(TypeError):
+            ops.embedding(t, w)
+        with pytest.raises(TypeError):
+            ops.embedding_grad(t, torch.ones(4, 3, device=DEV), 5)
+    with pytest.raises(ValueError):
+        ops.embedding(tok.cpu(), w)
+    with pytest.raises(RuntimeError):
+        ops.embedding(tok, torch.ones(3, 5, device=DEV).t())
+    gy = torch.ones(4, 3, device=DEV)
+    for out in (torch.zeros(5, 4, device=DEV), torch.zeros(4, 3, device=DEV), torch.zeros(5, 3), torch.zeros(3, 5, device=DEV).t()):
+        with pytest.raises(ValueError):
+            ops.embedding_grad(tok, gy, 5, out=out)
