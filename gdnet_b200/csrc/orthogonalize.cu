@@ -1596,9 +1596,11 @@ const char* launch_orthogonalize(const NsCall& call, Status* status, cudaStream_
   g.c = call.c[2];
   g.done = e.done;
   g.next_item = e.next_item;
-  // A pair's 256 x 256 tile needs half the operand traffic of a 128 x 128 one; with a side of 256 or less it would leave one
-  // or two pairs to work on each matrix.
-  const bool pair = g.k > 256 && !call.pairs;
+  // A pair's 256 x 256 tile needs half the operand traffic of a 128 x 128 one, but has four times its latency: worth it from three
+  // symmetric tiles for every four pairs on (32 of 512 x 512: 246 us against 264, six of 1024 x 1024: 249 against 255;
+  // 16 of 512 x 512: 207 against 176, three of 1024 x 1024: 229 against 210).
+  const int64_t k256 = (g.k + 255) / 256;
+  const bool pair = !call.pairs && g.k > 256 && batch * (k256 * (k256 + 1) / 2) >= 56;
   const int tile = pair ? 256 : 128;
   const int kt = (g.k + tile - 1) / tile, wt = (g.wide + tile - 1) / tile;
   g.tiles_sym = kt * (kt + 1) / 2;

@@ -50,10 +50,11 @@ __device__ __forceinline__ int64_t token_at(const void* tokens, int wide, int64_
 // lookup
 // ---------------------------------------------------------------------------------------
 // A row is covered by `tpr` threads (a power of two) in steps of V elements; a block of 256 threads holds 256 / tpr
-// row slots and each slot fetches four rows at a time, so that four ids and then four row pieces are in flight per
-// thread. An id outside [0, vocab) is never used as an index: its row is zero and the status word records it.
+// row slots and each slot fetches two rows at a time: two ids, then two row pieces in flight per thread (with four or eight a
+// batch of 32768 x 1024 bf16 took 22.5 and 30.7 us instead of 18.4: too few blocks to spread). The rows written are not kept in
+// cache before others, so the table stays there. An id outside [0, vocab) is never used as an index: its row is zero and the status word records it.
 constexpr int LOOKUP_THREADS = 256;
-constexpr int LOOKUP_ROWS = 4;
+constexpr int LOOKUP_ROWS = 2;
 
 template <typename T, int V, bool SCALED>
 __global__ void __launch_bounds__(LOOKUP_THREADS)
@@ -93,7 +94,9 @@ token_lookup_kernel(const void* __restrict__ tokens, int wide, int64_t n, const 
 #pragma unroll
         for (int i = 0; i < V; ++i) x[r].e[i] = from_f32<T>(to_f32(x[r].e[i]) * scale);
       }
-      *reinterpret_cast<Vec<T, V>*>(out + (row * vecs + v) * V) = x[r];
+      Vec<T, V>* to = reinterpret_cast<Vec<T, V>*>(out + (row * vecs + v) * V);
+      if constexpr (sizeof(Vec<T, V>) == 16) __stcs(reinterpret_cast<uint4*>(to), *reinterpret_cast<const uint4*>(&x[r]));
+      else *to = x[r];
     }
   }
 }
