@@ -1281,10 +1281,32 @@ void muon_update(at::TensorList params, at::TensorList grads, at::TensorList inf
 
   const auto here = c10::cuda::getCurrentCUDAStream(device.index());
   const auto side = groups.size() > 1 ? muon_side_stream(device.index()) : here;
+  struct Join {      // the side stream joins the caller's, also when a launch fails
+    c10::cuda::CUDAStream here, side;
+    ~Join() {
+      if (here == side) return;
+      try {
+        at::cuda::CUDAEvent done;
+        done.record(side);
+        done.block(here);
+      } catch (...) {
+      }
+    }
+  };
   if (groups.size() > 1) {
     at::cuda::CUDAEvent begun;
     begun.record(here);
     begun.block(side);
+  }
+  Join join{here, side};
+  // every workspace before the first launch: running out of memory leaves the parameters as they were
+  std::vector<Tensor> spaces(groups.size());
+  for (size_t k = 0; k < groups.size(); ++k) {
+    const Group& g = groups[k];
+    c10::cuda::CUDAStreamGuard on(k % 2 != 0 ? side : here);
+    const int64_t bytes = gd::ns_workspace_bytes(ns_group((int64_t)g.out.size(), g.rows, g.cols), g.rows, g.cols, (int)steps,
+                                                 g.type != at::kBFloat16);
+    if (bytes > 0) spaces[k] = at::empty({bytes}, params[0].options().dtype(at::kByte));
   }
   for (size_t k = 0; k < groups.size(); ++k) {
     const Group& g = groups[k];
@@ -1302,12 +1324,7 @@ void muon_update(at::TensorList params, at::TensorList grads, at::TensorList inf
     call.ends.decay = (float)(1.0 - lr * weight_decay);
     call.ends.step = (float)(lr * (update_scale >= 0.0 ? update_scale : 0.2 * std::sqrt((double)std::max(g.rows, g.cols))));
     const int64_t total = (int64_t)g.out.size(), group = ns_group(total, g.rows, g.cols);
-    const int64_t space_bytes = gd::ns_workspace_bytes(group, g.rows, g.cols, call.steps, call.pairs);
-    Tensor space;
-    if (space_bytes > 0) {
-      space = at::empty({space_bytes}, params[0].options().dtype(at::kByte));
-      call.workspace = space.data_ptr();
-    }
+    if (spaces[k].defined()) call.workspace = spaces[k].data_ptr();
     for (int64_t i0 = 0; i0 < total; i0 += group) {
       const int64_t count = std::min(group, total - i0);
       call.ends.batch = (int)count;
@@ -1317,11 +1334,6 @@ void muon_update(at::TensorList params, at::TensorList grads, at::TensorList inf
       std::copy_n(g.out.begin() + i0, count, call.ends.out);
       GD_LAUNCH(gd::launch_orthogonalize(call, status_ptr(params[0]), (k % 2 != 0 ? side : here).stream()));
     }
-  }
-  if (groups.size() > 1) {
-    at::cuda::CUDAEvent done;
-    done.record(side);
-    done.block(here);
   }
   for (size_t i = 0; i < n; ++i) {
     if (!params[i].is_inference()) params[i].unsafeGetTensorImpl()->bump_version();

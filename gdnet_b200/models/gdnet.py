@@ -74,10 +74,17 @@ class GDNet(nn.Module):
 
     # -- trunk ------------------------------------------------------------------------
 
+    embed_scale = 1.0
+
     def _embed(self, tokens: torch.Tensor) -> torch.Tensor:
-        if type(self.embed) is nn.Embedding:
-            return self.proj_in(ops.embedding(tokens, self.embed.weight, self.embed_scale))
-        return self.proj_in(self.embed(tokens) * self.embed_scale)      # a wrapped or replaced table
+        table = self.embed
+        w = table.weight if type(table) is nn.Embedding else None
+        if (w is not None and w.is_cuda and w.dtype in (torch.bfloat16, torch.float16, torch.float32)
+                and table.padding_idx is None and table.max_norm is None and not table.sparse and not table.scale_grad_by_freq
+                and not table._forward_hooks and not table._forward_pre_hooks):
+            return self.proj_in(ops.embedding(tokens, w, self.embed_scale))
+        x = table(tokens)                     # on CPU, or a table with options, hooks or a wrapper of its own
+        return self.proj_in(x if self.embed_scale == 1.0 else x * self.embed_scale)
 
     def one_cycle(self, fwd, side, sp_group=None, gate_sink=None, gate_mode=True, cycle=0):
         """All layers forward-step in order, then backward-step in reverse order.

@@ -808,7 +808,8 @@ def embedding_grad(tokens, grad, num_rows: int, scale: float = 1.0, out=None):
     if out is None:
         return K.token_grad(tokens if tokens.is_contiguous() else tokens.contiguous(), g, scale, num_rows, None)
     K.token_grad(tokens if tokens.is_contiguous() else tokens.contiguous(), g, scale, num_rows, out)
-    torch.autograd.graph.increment_version(out)
+    if not out.is_inference():
+        torch.autograd.graph.increment_version(out)
     return out
 
 

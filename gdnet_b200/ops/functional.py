@@ -176,8 +176,8 @@ def _ns_arguments(steps, coefficients, eps, what: str):
         raise ValueError(f"{what}: steps must be in [0, 100], got {steps}")
     if len(coefficients) != 3 or not all(math.isfinite(x) for x in coefficients):
         raise ValueError(f"{what}: three finite coefficients, got {coefficients}")
-    if not (eps > 0.0 and math.isfinite(eps)):
-        raise ValueError(f"{what}: eps must be positive, got {eps}")
+    if not (eps >= 1e-37 and math.isfinite(eps)):      # a matrix of zeros is divided by it
+        raise ValueError(f"{what}: eps must be at least 1e-37, got {eps}")
     _ns_check(coefficients, steps)
     return steps, coefficients, eps
 
@@ -231,7 +231,8 @@ def muon_update_(params, grads, momenta, *, lr: float, momentum: float = 0.95, n
     matrices ``(n, r, c)``, ``momenta`` the same in fp32; shapes may differ from entry to entry. ``scalars`` is a
     device tensor (projection coefficient, gradient scale) as the training engine keeps it. ``update_scale`` defaults to
     ``0.2 sqrt(max(r, c))``, which gives the update the size of an AdamW step of the same ``lr``. No two
-    entries may share memory."""
+    entries may share memory. Pass the parameters themselves rather than ``.data``: the copies of weights that the kernels
+    keep (FP8, folded) are renewed by the parameter's version."""
     params, grads, momenta = list(params), list(grads), list(momenta)
     infos = list(info_grads) if info_grads is not None else []
     if not (len(params) == len(grads) == len(momenta)) or (infos and len(infos) != len(params)):

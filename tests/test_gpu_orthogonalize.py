@@ -16,7 +16,7 @@ BF, FP, F32 = torch.bfloat16, torch.float16, torch.float32
 # one element, one row or column, sides under a tile, tile borders, tall and wide, both tile forms, many matrices
 @pytest.mark.parametrize("n,r,c", [(1, 1, 1), (3, 1, 70), (2, 90, 1), (1, 16, 16), (5, 33, 47), (2, 128, 128), (3, 129, 64),
                                    (1, 64, 1000), (2, 256, 256), (1, 256, 700), (2, 257, 257), (1, 300, 520), (1, 520, 301),
-                                   (2, 384, 1024), (1, 1030, 515), (1, 512, 512), (70, 40, 24)])
+                                   (2, 1, 2500), (1, 5000, 3), (2, 384, 1024), (1, 1030, 515), (1, 512, 512), (70, 40, 24)])
 @pytest.mark.parametrize("dtype", [BF, FP, F32])
 def test_orthogonalize(n, r, c, dtype):
     g = torch.Generator().manual_seed(r * 1000 + c)

@@ -196,3 +196,30 @@ def test_refusals():
     for out in (torch.zeros(5, 4, device=DEV), torch.zeros(4, 3, device=DEV), torch.zeros(5, 3), torch.zeros(3, 5, device=DEV).t()):
         with pytest.raises(ValueError):
             ops.embedding_grad(tok, gy, 5, out=out)
+
+
+def test_model_looks_up_through_the_table_op():
+    """GDNet's token path: the same rows as the module's, its gradient in autograd, and the module itself where it has hooks or
+    options."""
+    from gdnet_b200.model import GDNet
+    from gdnet_b200.ops import cuda as cu
+
+    torch.manual_seed(0)
+    m = GDNet(vocab_size=100, d_embed=32, d=32, n_layers=1, n_cycles=1, kernel_size=3, chunk_size=16, embed_scale=2.0).to(DEV)
+    tok = torch.randint(0, 100, (2, 16), device=DEV)
+    n0 = cu.launch_count()
+    y = m._embed(tok)
+    assert cu.launch_count() == n0 + 1
+    assert torch.equal(y, m.proj_in(m.embed(tok) * 2.0))
+    (g,) = torch.autograd.grad(y.sum(), m.embed.weight)
+    rows = torch.ones_like(y) @ m.proj_in.weight.detach()
+    assert torch.equal(g, ops.embedding_grad(tok, rows, m.embed.weight.shape[0], 2.0))
+    m.embed.padding_idx = 0
+    n0 = cu.launch_count()
+    assert torch.equal(m._embed(tok), y) and cu.launch_count() == n0
+    with torch.inference_mode():
+        m.embed.padding_idx = None
+        assert torch.equal(m._embed(tok), y)
+        out = torch.zeros(100, 32, device=DEV)
+        ops.embedding_grad(tok, torch.ones(2, 16, 32, device=DEV), 100, out=out)
+        assert float(out.sum()) == 2 * 16 * 32

@@ -91,7 +91,7 @@ def test_orthogonalize_refusals():
             ops.orthogonalize(bad)
     with pytest.raises(TypeError):
         ops.orthogonalize(x, out_dtype=torch.float64)
-    for kw in (dict(steps=-1), dict(steps=101), dict(eps=0.0), dict(eps=float("nan")), dict(coefficients=(1.0, 2.0)),
+    for kw in (dict(steps=-1), dict(steps=101), dict(eps=0.0), dict(eps=1e-50), dict(eps=float("nan")), dict(coefficients=(1.0, 2.0)),
                dict(coefficients=(1.0, float("inf"), 0.0)), dict(coefficients=(4.0, 0.0, 0.0)), dict(coefficients=(3.4445, -4.775, 9.0))):
         with pytest.raises(ValueError):
             ops.orthogonalize(x, **kw)
@@ -151,6 +151,11 @@ def test_model_scales_its_tokens():
     assert plain.state_dict().keys() == scaled.state_dict().keys()
     assert torch.equal(plain._embed(tok), plain.proj_in(plain.embed(tok)))
     assert torch.equal(scaled._embed(tok), scaled.proj_in(scaled.embed(tok) * 3.0))
+    seen = []
+    scaled.embed.register_forward_hook(lambda m, i, o: seen.append(o))
+    scaled._embed(tok)
+    assert len(seen) == 1
+    plain.double()._embed(tok)                              # other types go through the module, as before
 
 
 def test_engine_groups_and_state():
