@@ -159,8 +159,8 @@ const char* launch_token_lookup(const TokenLookupArgs& a, Status* status, cudaSt
 // Least-significant-digit radix sort by one cluster of sixteen blocks (512 warps), so that a pass needs no launch of
 // its own: every warp owns one contiguous slice of the list, counts its digits in a histogram of its own, and after
 // one exchange of the blocks' totals through distributed shared memory knows where each of its digits goes. Digits
-// are at most 9 bits (two passes up to a vocabulary of 2^18). Key and position travel as one 8-byte word: what bounds a pass is
-// the scattered stores of few SMs (with 8 blocks and two words 32768 tokens took 27 us, SORTTIME). A token outside [0, vocab) gets the key `vocab` and
+// are at most 9 bits (two passes up to a vocabulary of 2^18). Key and position travel as one 8-byte word: a pass of few SMs is bound by its stores
+// and by the latency of its steps (32768 tokens: 8 blocks and two words 27 us, 16 blocks and one word 19). A token outside [0, vocab) gets the key `vocab` and
 // sorts to the end, where the sums leave it out. The blocks behind the first cluster clear the dense gradient meanwhile.
 constexpr int SORT_CTAS = 16;       // more than 8 need leave (cudaFuncAttributeNonPortableClusterSizeAllowed)
 constexpr int SORT_THREADS = 1024;
@@ -235,18 +235,32 @@ token_sort_kernel(const void* __restrict__ tokens, int wide, int n, uint32_t voc
       }
     }
     __syncthreads();
-    // per digit: counts of the block's warps (one a lane) -> exclusive prefix, and the block's total
-#pragma unroll 4
-    for (int b = warp; b < bins; b += SORT_WARPS) {
-      const uint32_t c = hist[b * SORT_ROW + lane];
-      uint32_t incl = c;
+    // per digit: counts of the block's warps -> exclusive prefix, and the block's total. 2^split neighbouring lanes share a digit,
+    // each with an equal range of the warps (a warp per digit and a scan across its lanes took three times as long).
+    const int split = bins >= 512 ? 1 : 2, per = SORT_WARPS >> split;
+    for (int t = threadIdx.x; t < bins << split; t += SORT_THREADS) {
+      const int d = t >> split, piece = t & ((1 << split) - 1);
+      uint32_t* at = hist + d * SORT_ROW + piece * per;
+      uint32_t run = 0;
+      for (int w0 = 0; w0 < per; w0 += 8) {
+        uint32_t c[8];
 #pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const uint32_t t = __shfl_up_sync(0xffffffffu, incl, o);
-        if (lane >= o) incl += t;
+        for (int w = 0; w < 8; ++w) c[w] = at[w0 + w];
+#pragma unroll
+        for (int w = 0; w < 8; ++w) {
+          at[w0 + w] = run;
+          run += c[w];
+        }
       }
-      hist[b * SORT_ROW + lane] = incl - c;
-      if (lane == 31) total[b] = incl;
+      uint32_t before = 0, sum = run;
+      for (int o = 1; o < 1 << split; o <<= 1) {
+        const uint32_t other = __shfl_xor_sync(__activemask(), sum, o);
+        if (piece & o) before += other;
+        sum += other;
+      }
+      if (piece != 0)
+        for (int w = 0; w < per; ++w) at[w] += before;
+      if (piece == 0) total[d] = sum;
     }
     cluster_sync_all();
     // digit b starts at (all smaller digits of all blocks) + (digit b of the blocks before this one)
@@ -260,12 +274,14 @@ token_sort_kernel(const void* __restrict__ tokens, int wide, int n, uint32_t voc
       }
     }
     uint32_t incl = all;
+    if (warp * 32 < bins) {
 #pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const uint32_t t = __shfl_up_sync(0xffffffffu, incl, o);
-      if (lane >= o) incl += t;
+      for (int o = 1; o < 32; o <<= 1) {
+        const uint32_t t = __shfl_up_sync(0xffffffffu, incl, o);
+        if (lane >= o) incl += t;
+      }
+      if (lane == 31) warp_tot[warp] = incl;
     }
-    if (lane == 31) warp_tot[warp] = incl;
     __syncthreads();
     if ((int)threadIdx.x < bins) {
       uint32_t base = incl - all + before;
@@ -273,7 +289,8 @@ token_sort_kernel(const void* __restrict__ tokens, int wide, int n, uint32_t voc
       first[threadIdx.x] = base;
     }
     __syncthreads();
-    // place: equal digits of a warp's 32 keys keep their order (rank among the lower lanes)
+    // Place: equal digits of a warp's 32 keys keep their order (rank among the lower lanes). Neither ballots of the digit's bits
+    // instead of the match, nor ordering the block's keys in shared memory before they are written, was faster.
     for (int i0 = lo; i0 < hi; i0 += 32 * SORT_UNROLL) {
       if (!in_regs) fetch(i0);
       uint32_t same[SORT_UNROLL];                      // lanes with the same digit
@@ -302,7 +319,7 @@ token_sort_kernel(const void* __restrict__ tokens, int wide, int n, uint32_t voc
 // The sorted list is cut into chunks of `chunk` rows; `tpr` threads cover a row and walk one chunk. Each
 // thread's pieces of the next GRAD_RING rows are on their way into shared memory (asynchronous copies that only this thread
 // reads: no synchronisation), so the loop is short; with the rows in registers and unrolled, the code that ends an id was
-// there 8 or 16 times and fetching it took longer than the rows (35 and 90 us against RINGTIME for 32768 x 1024). An id whose rows all lie in one chunk is finished there. An id that runs over a
+// there 8 or 16 times and fetching it took longer than the rows (35 and 90 us against 30 for 32768 x 1024). An id whose rows all lie in one chunk is finished there. An id that runs over a
 // chunk's end leaves partial sums: slot 0 of a chunk holds the sum of the id that was already running when the chunk
 // began, slot 1 the sum of the id that runs on. token_grad_join_kernel adds those up in the order of the chunks.
 constexpr int GRAD_THREADS = 128;
@@ -691,6 +708,10 @@ static const char* grad_typed(const TokenGradArgs& a, const uint2* sorted, Statu
   return grad_as<T, 1, ADD>(a, sorted, status, st);
 }
 
+static size_t sort_smem(int bits) {
+  return (size_t)SORT_ROW * (1u << bits) * sizeof(uint32_t);
+}
+
 int64_t token_grad_sort_words(int64_t n) { return grad_is_direct(n) ? 0 : 4 * n; }
 
 const char* launch_token_grad(const TokenGradArgs& a, Status* status, cudaStream_t st) {
@@ -703,9 +724,9 @@ const char* launch_token_grad(const TokenGradArgs& a, Status* status, cudaStream
     while (need < 31 && (a.vocab >> need) != 0) ++need;           // keys are 0..vocab
     const int passes = (need + SORT_MAX_BITS - 1) / SORT_MAX_BITS;
     const int bits = (need + passes - 1) / passes;
-    const size_t smem = (size_t)SORT_ROW * (1u << bits) * sizeof(uint32_t);
+    const size_t smem = sort_smem(bits);
     if (cudaFuncSetAttribute(token_sort_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                             SORT_ROW * (1 << SORT_MAX_BITS) * (int)sizeof(uint32_t)) != cudaSuccess ||
+                             (int)sort_smem(SORT_MAX_BITS)) != cudaSuccess ||
         cudaFuncSetAttribute(token_sort_kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1) != cudaSuccess)
       return "token_sort: shared memory";
     uint2* list0 = reinterpret_cast<uint2*>(a.sort);
