@@ -6,18 +6,24 @@
 //
 // which moves every singular value s to s (a + b s^2 + c s^4) and keeps the singular vectors. Three products a step, the
 // first two symmetric: only the tiles on and above the diagonal of A and B are computed and stored, and what lies below is
-// read from above with the operand's other major order (a bit of the MMA instruction), so a step costs k (k + 1) w + k (k + 1) k + 2 k^2 w operations with k = min(r, c), w = max(r, c), against
-// 4 k^2 w + 2 k^3 without. Bound by the tensor cores from about k = 1024 on, by the latency of 3 x steps dependent
-// products below.
+// read from above with the operand's other major order (a bit of the MMA instruction). A step then costs
+// k (k + 1) w + k (k + 1) k + 2 k^2 w operations with k = min(r, c), w = max(r, c), against 4 k^2 w + 2 k^3.
+//
+// Matrices with a side of at most 256 (pairs: 128) stay in one cluster for the whole call (ns_small_kernel); larger ones go
+// tile by tile through one persistent kernel (ns_chain_body) between element-wise ends. Few matrices are bound by the
+// latency of 3 x steps dependent products (one 1024 x 1024: 0.21 ms), many by the tensor cores under the power cap and by the
+// epilogue of X <- a X + B X, which reads and writes X twice over (48 of 1024 x 1024: 1.5 ms, 0.69 PFLOP/s of the
+// operations above; four of 2048 x 4096: 1.3 ms, 0.92 PFLOP/s).
 //
 // Number format. Operands are fp16, scaled by 2^14: with the coefficients that the host admits the spectral norms of X, A
 // and B, and so their entries, stay below 3.9, and 3.9 * 2^14 < 65504, so entries down to 2^-28 keep all 11 bits.
 // X is held as hi + lo, two fp16 values (22 bits). With `pairs` off the products read the high parts only and the
 // linear term a X reads both: rounding errors then enter through B X alone, in the directions whose singular values
-// are already large (error of the result 5e-4 to 1.7e-3 of its norm, below the 1.7e-3 of rounding it to bf16; without the
+// are already large (error of the result 5e-4 to 1.7e-3 of its norm, at most that of rounding it to bf16; without the
 // low part in a X the noise of the large directions is amplified into the small ones, 3e-3 to 1e-1). With `pairs` on
 // every operand is a pair and a product is the three partial products hi hi + hi lo + lo hi (the result is as exact
-// as in fp32 arithmetic), at three times the tensor-core work and on single-CTA tiles, whose sums fit the registers. Sums are fp32 in TMEM; the norm is summed in fp64.
+// as in fp32 arithmetic), at three times the tensor-core work and on single-CTA tiles, whose sums fit the registers. Sums are
+// fp32 in TMEM; the norm is summed in fp64.
 #include "orthogonalize.h"
 
 #include <cuda_fp16.h>
@@ -60,13 +66,14 @@ __device__ __forceinline__ void tma_store_3d(const CUtensorMap* m, uint32_t src,
 // tiles per matrix says how far it is. So any number of resident blocks makes progress (two calls on two streams may share
 // the GPU), nothing is launched between the 3 x steps products, and the tiles of one product fill the gaps that
 // the end of another leaves. The order is: product by product, all matrices. (Windows of as many matrices as stay in L2 from
-// one product to the next were slower: 48 matrices of 1024 x 1024 take 1.69 ms as one window, 2.07 in windows of 8, whose ends
-// wait on one another.)
+// one product to the next were slower: 48 matrices of 1024 x 1024 took 1.69 ms as one window, 2.07 in windows of 8, whose ends
+// waited on one another.)
 //
 // A block: warp 10 fetches items, waits until what they read is written and hands them to the others; warp 0 loads operands
 // with bulk tensor copies into a ring of stages; warp 1 issues the MMAs into two accumulators in TMEM; warps 2..9
 // read the accumulator, add the linear term (its boxes are copied in while the MMAs run) and send 32 x 32 boxes
-// out with bulk stores. A diagonal tile of a symmetric product reads the same rows twice and loads them once. PAIR: a pair of CTAs on two SMs shares a
+// out with bulk stores. A diagonal tile of a symmetric product reads the same rows twice and loads them once.
+// PAIR: a pair of CTAs on two SMs shares a
 // 256 x 256 tile, each loading its half of both operands; otherwise a CTA has a 128 x 128 tile of its own.
 constexpr int NS_BK = 64;                       // K elements per stage: one 128-byte swizzle row
 constexpr int NS_EPI_WARPS = 8;
@@ -940,10 +947,12 @@ ns_end_kernel(const __grid_constant__ NsEnds e) {
 // the fp32 X in TMEM, its fp16 operands in shared memory. A tile of X lies as k rows of 128-byte pieces, which is the K-major
 // operand of A = X X^T and, read as rows of the reduction, the MN-major operand of B X. X in TMEM is stored times a, so that
 // the MMAs of B X add to the linear term in place (with pairs B X has columns of its own and is added in registers: the
-// tensor core cuts a sum where fp32 rounds it, and a X is several times the result). The slices' shares of A are summed through distributed shared memory:
+// tensor core cuts a sum where fp32 rounds it, and a X is several times the result).
+// The slices' shares of A are summed through distributed shared memory:
 // every CTA adds up some of the rows, in the order of the CTAs, and hands them to all. What bounds this kernel is the chain of
-// 3 x steps products with an exchange of operands between them (about 2.5 us a step in one CTA), not work or traffic;
-// one 128 x 512 matrix took 111 us as tiles handed out by ns_chain_body.
+// 3 x steps products with an exchange of operands between them (128 x 256: 35 us a call, 4 us a step; 256 x 256: 98 us, 17 us
+// a step, most of it the exchange of A), not work or traffic; as tiles handed out by ns_chain_body one 128 x 512 matrix
+// took 111 us instead of 50.
 constexpr int SM_THREADS = 512;                      // 16 warps: four share the rows of a lane quarter and split its columns
 constexpr int SM_PANEL = 128 * 128;                 // 128 rows x 64 fp16
 

@@ -51,8 +51,9 @@ __device__ __forceinline__ int64_t token_at(const void* tokens, int wide, int64_
 // ---------------------------------------------------------------------------------------
 // A row is covered by `tpr` threads (a power of two) in steps of V elements; a block of 256 threads holds 256 / tpr
 // row slots and each slot fetches two rows at a time: two ids, then two row pieces in flight per thread (with four or eight a
-// batch of 32768 x 1024 bf16 took 22.5 and 30.7 us instead of 18.4: too few blocks to spread). The rows written are not kept in
-// cache before others, so the table stays there. An id outside [0, vocab) is never used as an index: its row is zero and the status word records it.
+// batch of 32768 x 1024 bf16 took 22.5 and 30.7 us instead of 18.4, whose bytes need 13: too few blocks to spread). The rows
+// written are not kept in cache before others, so the table stays there. An id outside [0, vocab) is never used as an
+// index: its row is zero and the status word records it.
 constexpr int LOOKUP_THREADS = 256;
 constexpr int LOOKUP_ROWS = 2;
 
@@ -159,9 +160,10 @@ const char* launch_token_lookup(const TokenLookupArgs& a, Status* status, cudaSt
 // Least-significant-digit radix sort by one cluster of sixteen blocks (512 warps), so that a pass needs no launch of
 // its own: every warp owns one contiguous slice of the list, counts its digits in a histogram of its own, and after
 // one exchange of the blocks' totals through distributed shared memory knows where each of its digits goes. Digits
-// are at most 9 bits (two passes up to a vocabulary of 2^18). Key and position travel as one 8-byte word: a pass of few SMs is bound by its stores
-// and by the latency of its steps (32768 tokens: 8 blocks and two words 27 us, 16 blocks and one word 19). A token outside [0, vocab) gets the key `vocab` and
-// sorts to the end, where the sums leave it out. The blocks behind the first cluster clear the dense gradient meanwhile.
+// are at most 9 bits (two passes up to a vocabulary of 2^18). Key and position travel as one 8-byte word: a pass of few SMs is
+// bound by its stores and by the latency of its steps (32768 tokens: 8 blocks and two words 27 us, 16 blocks and one word 19).
+// A token outside [0, vocab) gets the key `vocab` and sorts to the end, where the sums leave it out. The blocks behind the
+// first cluster clear the dense gradient meanwhile.
 constexpr int SORT_CTAS = 16;       // more than 8 need leave (cudaFuncAttributeNonPortableClusterSizeAllowed)
 constexpr int SORT_THREADS = 1024;
 constexpr int SORT_WARPS = SORT_THREADS / 32;
@@ -319,9 +321,10 @@ token_sort_kernel(const void* __restrict__ tokens, int wide, int n, uint32_t voc
 // The sorted list is cut into chunks of `chunk` rows; `tpr` threads cover a row and walk one chunk. Each
 // thread's pieces of the next GRAD_RING rows are on their way into shared memory (asynchronous copies that only this thread
 // reads: no synchronisation), so the loop is short; with the rows in registers and unrolled, the code that ends an id was
-// there 8 or 16 times and fetching it took longer than the rows (35 and 90 us against 30 for 32768 x 1024). An id whose rows all lie in one chunk is finished there. An id that runs over a
-// chunk's end leaves partial sums: slot 0 of a chunk holds the sum of the id that was already running when the chunk
-// began, slot 1 the sum of the id that runs on. token_grad_join_kernel adds those up in the order of the chunks.
+// there 8 or 16 times and fetching it took longer than the rows (35 and 90 us against 30 for 32768 x 1024, whose bytes need 21).
+// An id whose rows all lie in one chunk is finished there. An id that runs over a chunk's end leaves partial sums: slot 0
+// of a chunk holds the sum of the id that was already running when the chunk began, slot 1 the sum of the id that runs
+// on. token_grad_join_kernel adds those up in the order of the chunks.
 constexpr int GRAD_THREADS = 128;
 constexpr int GRAD_INFLIGHT = 8;
 constexpr int GRAD_MAX_CHUNK = 64;
