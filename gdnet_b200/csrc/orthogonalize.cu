@@ -138,6 +138,18 @@ __device__ __forceinline__ uint32_t ns_try_wait_cluster(uint32_t bar, uint32_t p
       : "memory");
   return ok;
 }
+// Without the time that a try_wait may be suspended for.
+__device__ __forceinline__ uint32_t ns_test_wait_cluster(uint32_t bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "mbarrier.test_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(bar), "r"(parity)
+      : "memory");
+  return ok;
+}
 __device__ __forceinline__ void ns_put_remote(uint32_t cluster_addr, uint4 v) {
   asm volatile("st.shared::cluster.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(cluster_addr), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
 }
@@ -191,7 +203,7 @@ __device__ __forceinline__ NsItem ns_next_item(NsBars* bars, int slot_no, Status
 __device__ __forceinline__ bool ns_item_there(NsBars* bars, int slot_no) {
   uint32_t ok = 0;
   if ((threadIdx.x & 31) == 0)
-    ok = ns_try_wait_cluster(smem_u32(&bars->item_full[slot_no & (NS_RING - 1)]), (slot_no / NS_RING) & 1);
+    ok = ns_test_wait_cluster(smem_u32(&bars->item_full[slot_no & (NS_RING - 1)]), (slot_no / NS_RING) & 1);
   return __shfl_sync(0xffffffffu, ok, 0) != 0;
 }
 
@@ -806,7 +818,8 @@ __device__ __forceinline__ void momentum_step(const NsEnds& e, float kt, float k
 }
 
 // u (fp32, row pitch ld) of every matrix and the blocks' partial sums of u^2. Without momentum u is the input itself.
-template <int V>
+// (MOMENTUM is a parameter of the code because the loads of its inputs cost registers, and those cost blocks per SM.)
+template <int V, bool MOMENTUM>
 __global__ void __launch_bounds__(ENDS_THREADS)
 ns_begin_kernel(const __grid_constant__ NsEnds e) {
   __shared__ double red[ENDS_THREADS / 32];
@@ -835,7 +848,7 @@ ns_begin_kernel(const __grid_constant__ NsEnds e) {
         const int r = r0 + q * groups + group;
         if (r >= e.rows) continue;
         g[q] = load_vec<V>(gt, e.grad_dtype, (int64_t)r * e.grad_ld + c);
-        if (e.momentum) {
+        if (MOMENTUM) {
           m[q] = *reinterpret_cast<const VecF<V>*>(mom + (int64_t)r * e.cols + c);
           if (gi != nullptr) f[q] = load_vec<V>(gi, e.grad_dtype, (int64_t)r * e.grad_ld + c);
         }
@@ -845,7 +858,7 @@ ns_begin_kernel(const __grid_constant__ NsEnds e) {
         const int r = r0 + q * groups + group;
         if (r >= e.rows) continue;
         VecF<V> u = g[q];
-        if (e.momentum) {
+        if (MOMENTUM) {
           momentum_step<V>(e, kt, ki, gi != nullptr, u, f[q], m[q]);
           *reinterpret_cast<VecF<V>*>(mom + (int64_t)r * e.cols + c) = m[q];
         }
@@ -1482,7 +1495,8 @@ static NsSpace ns_space(int64_t batch, int64_t rows, int64_t cols) {
 
 template <int V>
 static void ns_begin(const NsEnds& e, int norm_blocks, int blocks, cudaStream_t st) {
-  ns_begin_kernel<V><<<dim3(norm_blocks, e.batch), ENDS_THREADS, 0, st>>>(e);
+  if (e.momentum) ns_begin_kernel<V, true><<<dim3(norm_blocks, e.batch), ENDS_THREADS, 0, st>>>(e);
+  else ns_begin_kernel<V, false><<<dim3(norm_blocks, e.batch), ENDS_THREADS, 0, st>>>(e);
   ns_scale_kernel<V><<<dim3(blocks, e.batch), ENDS_THREADS, 0, st>>>(e, norm_blocks);
 }
 

@@ -11,7 +11,7 @@
 namespace gd {
 
 constexpr int NS_MAX_BATCH = 64;       // matrices of one shape per call: their addresses travel in the kernel arguments
-constexpr int NS_NORM_BLOCKS = 64;     // partial sums of a matrix's norm
+constexpr int NS_NORM_BLOCKS = 256;    // partial sums of a matrix's norm
 
 // Element-wise ends of a call: what the matrices are made from and where the result goes.
 struct NsEnds {
