@@ -11,7 +11,7 @@
 //
 // Matrices with a side of at most 256 (pairs: 128) stay in one cluster for the whole call (ns_small_kernel); larger ones go
 // tile by tile through one persistent kernel (ns_chain_body) between element-wise ends. Few matrices are bound by the
-// latency of 3 x steps dependent products (one 1024 x 1024: 0.21 ms), many by the tensor cores under the power cap and by the
+// latency of 3 x steps dependent products (one 1024 x 1024: 0.16 ms), many by the tensor cores under the power cap and by the
 // epilogue of X <- a X + B X, which reads and writes X twice over (48 of 1024 x 1024: 1.5 ms, 0.69 PFLOP/s of the
 // operations above; four of 2048 x 4096: 1.3 ms, 0.92 PFLOP/s).
 //
@@ -1545,17 +1545,15 @@ static const char* launch_small(const NsCall& call, Status* status, cudaStream_t
 }
 
 // Row blocks of a matrix that one cluster keeps, 0 for the others. One block of 128 rows: 8 CTAs with slices of 256 columns, or, with
-// pairs, 16 with slices of 128. Two blocks: 4 or 8 CTAs with slices of 64 columns; pairs do not fit.
-// With two blocks the exchange of A weighs more, so they are worth it only while all clusters run at once (fewer of the larger ones
-// do): 32 matrices of 256 x 256 (4 CTAs each) 101 us against 143 in ns_chain_body, 64 of them 198 against 163; 8 of 256 x 512
-// (8 CTAs) 112 against 133, 16 of them 221 against 143; 8 of 200 x 1000 (16 CTAs) 252 against 145.
+// pairs, 16 with slices of 128. Two blocks: 4 CTAs with slices of 64 columns; pairs do not fit.
+// With two blocks the exchange of A weighs more, so they are worth it only up to 256 x 256 and while all clusters run at once: 32
+// matrices 107 us against 131 in ns_chain_body, one of them 99 against 100, 64 of them 198 against 157; in 8 CTAs one of 256 x 512
+// took 111 against 107, 8 of them 113 against 112.
 static int ns_small_blocks(int64_t batch, int64_t rows, int64_t cols, int steps, int pairs) {
   const int64_t k = rows < cols ? rows : cols, wide = rows < cols ? cols : rows;
   if (steps == 0) return 0;
   if (k <= 128 && wide <= 2048) return 1;
-  int64_t ctas = 1;
-  while (ctas * 64 < wide) ctas *= 2;
-  return k <= 256 && !pairs && ((ctas <= 4 && batch * ctas <= 128) || (ctas == 8 && batch <= 8)) ? 2 : 0;
+  return wide <= 256 && batch <= 32 && !pairs ? 2 : 0;
 }
 
 int64_t ns_workspace_bytes(int64_t batch, int64_t rows, int64_t cols, int steps, int pairs) {
@@ -1619,11 +1617,12 @@ const char* launch_orthogonalize(const NsCall& call, Status* status, cudaStream_
   g.c = call.c[2];
   g.done = e.done;
   g.next_item = e.next_item;
-  // A pair's 256 x 256 tile needs half the operand traffic of a 128 x 128 one, but has four times its latency: worth it from three
-  // symmetric tiles for every four pairs on (32 of 512 x 512: 246 us against 264, six of 1024 x 1024: 249 against 255;
-  // 16 of 512 x 512: 207 against 176, three of 1024 x 1024: 229 against 210).
-  const int64_t k256 = (g.k + 255) / 256;
-  const bool pair = !call.pairs && g.k > 256 && batch * (k256 * (k256 + 1) / 2) >= 56;
+  // A pair's 256 x 256 tile needs half the operand traffic of a 128 x 128 one, but has four times its latency: worth it where a step
+  // has some three tiles for every pair (32 of 512 x 512: 238 us against 255 with single tiles, 16 of 512 x 2048: 364 against 416,
+  // six of 1024 x 1024: 244 against 250; ten of 768 x 768: 233 against 219, 20 of 512 x 512: 211 against 187) or where the sums
+  // are long (one 1400 x 1400: 228 against 251, one 1536 x 1536: 237 against 270; one 1024 x 1024: 191 against 157).
+  const int64_t k256 = (g.k + 255) / 256, wide256 = (g.wide + 255) / 256;
+  const bool pair = !call.pairs && g.k > 256 && (batch * (k256 * (k256 + 1) + k256 * wide256) >= 210 || g.k >= 1280);
   const int tile = pair ? 256 : 128;
   const int kt = (g.k + tile - 1) / tile, wt = (g.wide + tile - 1) / tile;
   g.tiles_sym = kt * (kt + 1) / 2;
@@ -1660,8 +1659,13 @@ const char* launch_orthogonalize(const NsCall& call, Status* status, cudaStream_
     auto kernel = call.pairs ? ns_chain_split_kernel : (pair ? ns_chain_pair_kernel : ns_chain_kernel);
     const int smem = call.pairs ? NsShape<true>::SMEM : NsShape<false>::SMEM;
     if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) return "orthogonalize: shared memory";
-    const int most = (int)(batch * g.tiles_x < units ? batch * g.tiles_x : units);      // no product has more tiles at once than that
-    kernel<<<(pair ? 2 : 1) * most, NS_THREADS, smem, st>>>(g, status);
+    // No product has more tiles at once than batch x tiles_x, but a CTA that finishes one has its next item, of a later
+    // product, in hand already, and its loads wait while others stand idle: with four CTAs a tile the next product's items
+    // are with CTAs that have nothing else to do (one 1024 x 1024: 206 us with one a tile, 164 with two, 156 with four, 156
+    // with the whole device; 1030 x 515 in pairs of fp16: 271, 232, 232, 232). What is left stays free for a second shape.
+    const int64_t most = 4 * batch * g.tiles_x;
+    const int count = (int)(most < units ? most : units);
+    kernel<<<(pair ? 2 : 1) * count, NS_THREADS, smem, st>>>(g, status);
   }
   e.x_hi = x[g.steps & 1];
   e.x_lo = x[g.steps & 1] + lo_x;
