@@ -49,7 +49,7 @@ struct NsPlan {
   uint32_t* next_item;
 };
 
-// A call whose matrices have a side of at most 128 (see ns_small_kernel).
+// A call whose matrices stay in one cluster each (see ns_small_kernel).
 struct NsSmall {
   int k, wide, tall, steps;
   int ctas, slice;                     // CTAs per matrix, columns of X per CTA

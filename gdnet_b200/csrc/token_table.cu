@@ -4,8 +4,8 @@
 //   gradient   dW[v, :] (+)= scale * sum over {t : tok_t = v} of dY[t, :]
 //
 // The gradient sorts the token positions by id (stable, so the rows of one id stay in the order of the batch), then
-// walks the sorted list in chunks and sums the rows of each id in fp32 registers. No atomics: the same inputs give
-// the same bits. Both directions move every row once and are bound by memory bandwidth; the sort moves 16 bytes a
+// walks the sorted list in chunks and sums the rows of each id in fp32 registers. An element is written once, or added once to
+// what stood there: the same inputs give the same bits. Both directions move every row once and are bound by memory bandwidth; the sort moves 16 bytes a
 // token and is bound by the latency of its few dependent steps.
 #include "kernels.h"
 

@@ -103,13 +103,22 @@ def _check_tokens(tokens, like, what: str) -> None:
         raise ValueError(f"{what}: tokens are on {tokens.device}, the rows on {like.device}")
 
 
+def _share_memory(a, b) -> bool:
+    """Whether the memory ranges of two tensors meet."""
+    if a.numel() == 0 or b.numel() == 0:
+        return False
+    span = [(t.data_ptr(), t.data_ptr() + (1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride()))) * t.element_size()) for t in (a, b)]
+    return span[0][0] < span[1][1] and span[1][0] < span[0][1]
+
+
 def embedding(tokens, weight, scale: float = 1.0):
     """``scale * weight[tokens]``: ``tokens`` (any shape, int64 or int32) to ``tokens.shape + (width,)`` in the type of
     ``weight (vocab, width)`` (bf16, fp16 or fp32), multiplied in fp32 and rounded once.
 
     Differentiable in ``weight``. On CUDA the gradient is :func:`embedding_grad`: with a ``main_grad`` installed by the
     training engine it is added there in fp32 and autograd gets none. An id outside the table gives a row of zeros, no
-    gradient, and a bad-argument code in the kernel status word (on CPU an ``IndexError``)."""
+    gradient, and a bad-argument code in the kernel status word (on CPU an ``IndexError``). Like every backward pass of torch,
+    one that a CUDA graph captures needs the table to be in no live graph that was made outside the capture."""
     if weight.is_cuda:      # checked in the binding
         return _cuda().embedding(tokens, weight, scale)
     if weight.dim() != 2 or weight.dtype not in _TABLE_TYPES:
@@ -125,8 +134,8 @@ def embedding_grad(tokens, grad, num_rows: int, scale: float = 1.0, out=None):
 
     Without ``out`` a dense gradient in the type of ``grad`` (summed in fp32, rounded once; rows of absent ids are zero).
     With ``out`` (fp32, contiguous) the sums are added to it, only the rows of ids that occur are touched, and ``out``
-    is returned. The rows of an id are summed in a fixed order: the same inputs give the same bits. Ids outside
-    the table are left out."""
+    is returned; it must not share memory with ``grad`` or ``tokens``. The rows of an id are summed in a fixed order: the same
+    inputs give the same bits. Ids outside the table are left out."""
     if grad.dtype not in _TABLE_TYPES or grad.dim() < 1:
         raise TypeError(f"embedding_grad: grad must be bf16, fp16 or fp32, got {grad.dtype}")
     _check_tokens(tokens, grad, "embedding_grad")
@@ -140,6 +149,8 @@ def embedding_grad(tokens, grad, num_rows: int, scale: float = 1.0, out=None):
             raise ValueError("embedding_grad: out must be a contiguous fp32 tensor on the gradient's device")
         if tuple(out.shape) != (num_rows, grad.shape[-1]):
             raise ValueError(f"embedding_grad: out {tuple(out.shape)} is not ({num_rows}, {grad.shape[-1]})")
+        if _share_memory(out, grad) or _share_memory(out, tokens):
+            raise ValueError("embedding_grad: out shares memory with grad or tokens")
     if _on_gpu(grad):
         return _cuda().embedding_grad(tokens, grad, num_rows, float(scale), out)
     return ref.embedding_grad(tokens, grad, num_rows, float(scale), out)

@@ -72,6 +72,17 @@ def test_table_refusals():
         ops.embedding(tok, w.to("meta"))
 
 
+def test_gradient_refuses_its_own_memory():
+    tok = torch.tensor([2, 0, 1, 2])
+    flat = torch.zeros(40)
+    for gy, out in ((flat[:12].view(4, 3), flat[11:26].view(5, 3)), (flat[:24].view(4, 6)[:, ::2], flat[20:35].view(5, 3))):
+        with pytest.raises(ValueError):
+            ops.embedding_grad(tok, gy, 5, out=out)
+    with pytest.raises(ValueError):
+        ops.embedding_grad(flat[:8].view(torch.int64), flat[20:32].view(4, 3), 5, out=flat[7:22].view(5, 3))
+    ops.embedding_grad(tok, flat[:12].view(4, 3), 5, out=flat[12:27].view(5, 3))
+
+
 @pytest.mark.parametrize("n,r,c", [(2, 16, 16), (1, 5, 33), (3, 40, 12), (1, 1, 1)])
 def test_orthogonalize_reference(n, r, c):
     g = torch.Generator().manual_seed(2)
