@@ -306,3 +306,17 @@ def test_muon_shapes_side_by_side():
     torch.cuda.synchronize()
     for a, b in zip(ps + ms, one[0] + one[1]):
         assert torch.equal(a, b)
+
+
+# pairs of CTAs: long sums of one matrix, and many small matrices, with sides off the tiles; a bank just past those that stay in clusters
+@pytest.mark.parametrize("n,r,c", [(1, 1281, 1300), (1, 1500, 1283), (1, 1290, 2049), (24, 257, 300), (22, 600, 261), (33, 256, 200),
+                                   (32, 200, 256), (60, 130, 258)])
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_pairs_of_blocks(n, r, c, dtype):
+    g = torch.Generator().manual_seed(r * 1000 + c)
+    x = gradient_like(g, n, r, c, DEV).to(dtype)
+    got = ops.orthogonalize(x)
+    want, tol = orthogonalize_bound(x.cpu(), dtype)
+    for i in range(n):
+        assert rel(got[i], want[i]) <= 2 * tol, (i, rel(got[i], want[i]), tol)
+    assert torch.equal(got, ops.orthogonalize(x))
